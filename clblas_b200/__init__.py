@@ -26,6 +26,9 @@ clblasUpper, clblasLower = 0, 1
 clblasUnit, clblasNonUnit = 0, 1
 clblasLeft, clblasRight = 0, 1
 
+# element types of the narrow-type operators (no reference counterpart)
+clblasB200Float32, clblasB200Float16, clblasB200Bfloat16 = 0, 1, 2
+
 # status codes (src/clBLAS.h:123-155)
 STATUS = {
     "clblasSuccess": 0, "clblasInvalidValue": -30, "clblasInvalidCommandQueue": -36,
@@ -194,6 +197,11 @@ def _load() -> ctypes.CDLL:
         f = getattr(lib, name)
         f.argtypes = [i, i, i, i, i, sz, sz, ft, vp, sz, sz, vp, sz, sz, vp, i, u, pvp, u, pvp, pvp]
         f.restype = i
+    lib.clblasB200QuantizeI8.argtypes = [i, i, sz, sz, i, vp, sz, sz, vp, sz, sz, vp, sz] + tail
+    lib.clblasB200QuantizeI8.restype = i
+    lib.clblasB200I8gemm.argtypes = [i, i, i, sz, sz, sz, ctypes.c_float, vp, sz, sz, vp, sz, vp, sz, sz, vp, sz,
+                                     ctypes.c_float, i, vp, sz, sz] + tail
+    lib.clblasB200I8gemm.restype = i
     return lib
 
 
@@ -206,7 +214,8 @@ EXPORTS = ["clblasSetup", "clblasTeardown", "clblasGetVersion", "clblasSgemm", "
            "clblasSsymm", "clblasDsymm", "clblasCgemm", "clblasZgemm", "clblasCtrsm", "clblasZtrsm", "clblasB200SgemmHost", "clblasB200DgemmHost", "clblasB200StrsmHost", "clblasB200DtrsmHost"] + MATRIX_HELPERS + COMPLEX_SYM + ["clblasCtrmm", "clblasZtrmm"] + [
     "clblasB200LastGemmVariant", "clblasB200WorkspaceAllocCount", "clblasB200NoAllocLimits", "clblasB200CommGetUniqueId",
     "clblasB200CommInitRank", "clblasB200CommInitAll", "clblasB200CommDestroy", "clblasB200CommInfo", "clblasB200PanelPlan",
-    "clblasB200SgemmSharded", "clblasB200DgemmSharded", "clblasB200StrsmSharded", "clblasB200DtrsmSharded"]
+    "clblasB200SgemmSharded", "clblasB200DgemmSharded", "clblasB200StrsmSharded", "clblasB200DtrsmSharded",
+    "clblasB200QuantizeI8", "clblasB200I8gemm"]
 
 
 def _ptr(x) -> Optional[int]:
@@ -280,6 +289,24 @@ def clblasDgemm(order, transA, transB, M, N, K, alpha, A, offA, lda, B, offB, ld
                 queues=None, wait=None, events=None) -> int:
     return _gemm(lib.clblasDgemm, order, transA, transB, M, N, K, alpha, A, offA, lda, B, offB, ldb, beta,
                  C, offC, ldc, queues, wait, events)
+
+
+def clblasB200QuantizeI8(order, side, M, N, typeX, X, offX, ldx, Q, offQ, ldq, scale, offScale,
+                         queues=None, wait=None, events=None) -> int:
+    """X (M x N, of ``clblasB200Float32`` / ``Float16`` / ``Bfloat16``) in signed 8-bit integers Q with one float32 scale per row
+    (``clblasLeft``: X ~ diag(scale) Q) or per column (``clblasRight``)."""
+    nq, q, nw, w, e = _queues_events(queues, wait, events)
+    return lib.clblasB200QuantizeI8(order, side, M, N, typeX, _ptr(X), offX, ldx, _ptr(Q), offQ, ldq, _ptr(scale), offScale,
+                                    nq, q, nw, w, e)
+
+
+def clblasB200I8gemm(order, transA, transB, M, N, K, alpha, A, offA, lda, scaleA, offScaleA, B, offB, ldb, scaleB, offScaleB,
+                     beta, typeC, C, offC, ldc, queues=None, wait=None, events=None) -> int:
+    """C <- alpha diag(scaleA) op(A) op(B) diag(scaleB) + beta C: A and B signed 8-bit integers, C of ``typeC``; the scales
+    (float32, ``None``: ones) have M and N elements."""
+    nq, q, nw, w, e = _queues_events(queues, wait, events)
+    return lib.clblasB200I8gemm(order, transA, transB, M, N, K, alpha, _ptr(A), offA, lda, _ptr(scaleA), offScaleA,
+                                _ptr(B), offB, ldb, _ptr(scaleB), offScaleB, beta, typeC, _ptr(C), offC, ldc, nq, q, nw, w, e)
 
 
 def _host_addr(x) -> Optional[int]:

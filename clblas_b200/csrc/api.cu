@@ -728,6 +728,131 @@ clblasStatus symm_entry(clblasOrder order, clblasSide side, clblasUplo uplo, siz
     return record_out(nq, queues, events);
 }
 
+// ---- narrow types ---------------------------------------------------------------------------------------------------
+
+bool valid_type(int t) { return t == clblasB200Float32 || t == clblasB200Float16 || t == clblasB200Bfloat16; }
+size_t type_size(int t) { return t == clblasB200Float32 ? 4 : 2; }
+
+// Device that holds `ptr`; -1 when the driver does not know.  (Asked of the result's buffer and not of the stream: the stream's
+// device cannot be queried while the stream is being captured.)
+typedef int (*PointerGetAttributeFn)(void*, int, unsigned long long);
+int device_of(const void* ptr)
+{
+    static PointerGetAttributeFn fn = [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuPointerGetAttribute", &f, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) f = nullptr;
+        return reinterpret_cast<PointerGetAttributeFn>(f);
+    }();
+    constexpr int kDeviceOrdinal = 9;                      // CU_POINTER_ATTRIBUTE_DEVICE_ORDINAL
+    int d = -1;
+    if (!fn || fn(&d, kDeviceOrdinal, (unsigned long long)(uintptr_t)ptr) != 0) return -1;
+    return d;
+}
+
+// Makes the device that holds the result current for the length of a call.
+struct ResultDevice {
+    int before = -1, device = -1;
+    explicit ResultDevice(const void* result)
+    {
+        if (cudaGetDevice(&before) != cudaSuccess) { cudaGetLastError(); before = -1; }
+        device = device_of(result);
+        if (device < 0) device = before;
+        if (device != before && cudaSetDevice(device) != cudaSuccess) { cudaGetLastError(); device = before; }
+    }
+    ~ResultDevice() { if (device != before && before >= 0) cudaSetDevice(before); }
+};
+
+bool on_other_device(const void* ptr, int device)
+{
+    const int d = device_of(ptr);
+    return d >= 0 && d != device;
+}
+
+// A vector of n FP32 values at buf + off.
+clblasStatus check_f32_vector(const void* buf, size_t off, size_t n, int device, clblasStatus invalid, clblasStatus insufficient)
+{
+    size_t avail = 0;
+    if (buf == nullptr || !bytes_after(buf, &avail) || on_other_device(buf, device)) return invalid;
+    return off > avail / 4 || n > avail / 4 - off ? insufficient : clblasSuccess;
+}
+
+clblasStatus quantize_entry(clblasOrder order, clblasSide side, size_t M, size_t N, int type, const void* X, size_t offX, size_t ldx,
+                            void* Q, size_t offQ, size_t ldq, void* scale, size_t offS,
+                            unsigned nq, clblasQueue* queues, unsigned nev, const clblasEvent* wait, clblasEvent* events)
+{
+    if (X == nullptr) return clblasInvalidMatA;
+    if (Q == nullptr) return clblasInvalidMatB;
+    if (scale == nullptr) return clblasInvalidVecX;
+    if (order != clblasRowMajor && order != clblasColumnMajor) return clblasInvalidValue;
+    if ((unsigned)side > 1u || !valid_type(type)) return clblasInvalidValue;
+    clblasStatus st;
+    if ((st = check_matrix_sizes(type_size(type), order, clblasNoTrans, M, N, X, offX, ldx, SET_A)) != clblasSuccess) return st;
+    if ((st = check_matrix_sizes(1, order, clblasNoTrans, M, N, Q, offQ, ldq, SET_B)) != clblasSuccess) return st;
+    if ((st = check_queues(nq, queues)) != clblasSuccess) return st;
+    if ((st = check_events(nev, wait)) != clblasSuccess) return st;
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(queues[0]);
+    ResultDevice dev(Q);
+    if (on_other_device(X, dev.device)) return clblasInvalidMatA;
+    if ((st = check_f32_vector(scale, offS, side == clblasLeft ? M : N, dev.device, clblasInvalidVecX, clblasInsufficientMemVecX)) != clblasSuccess) return st;
+    if ((st = wait_all(s, nev, wait)) != clblasSuccess) return st;
+
+    const bool row = order == clblasRowMajor;
+    const cudaError_t e = quantize_i8(type, row == (side == clblasLeft), X, offX, ldx, static_cast<signed char*>(Q) + offQ, ldq,
+                                      static_cast<float*>(scale) + offS, row ? M : N, row ? N : M, s);
+    if (e != cudaSuccess) { cudaGetLastError(); return from_cuda(e); }
+    return record_out(nq, queues, events);
+}
+
+clblasStatus i8gemm_entry(clblasOrder order, clblasTranspose transA, clblasTranspose transB, size_t M, size_t N, size_t K, float alpha,
+                          const void* A, size_t offA, size_t lda, const void* scaleA, size_t offSA,
+                          const void* B, size_t offB, size_t ldb, const void* scaleB, size_t offSB,
+                          float beta, int type, void* C, size_t offC, size_t ldc,
+                          unsigned nq, clblasQueue* queues, unsigned nev, const clblasEvent* wait, clblasEvent* events)
+{
+    if (A == nullptr) return clblasInvalidMatA;
+    if (B == nullptr) return clblasInvalidMatB;
+    if (C == nullptr) return clblasInvalidMatC;
+    if (order != clblasRowMajor && order != clblasColumnMajor) return clblasInvalidValue;
+    if ((unsigned)transA > 2u || (unsigned)transB > 2u || !valid_type(type)) return clblasInvalidValue;
+    clblasStatus st;
+    if (K != 0) {
+        if ((st = check_matrix_sizes(1, order, transA, M, K, A, offA, lda, SET_A)) != clblasSuccess) return st;
+        if ((st = check_matrix_sizes(1, order, transB, K, N, B, offB, ldb, SET_B)) != clblasSuccess) return st;
+    }
+    if ((st = check_matrix_sizes(type_size(type), order, clblasNoTrans, M, N, C, offC, ldc, SET_C)) != clblasSuccess) return st;
+    if (K > 131071) return clblasInvalidDim;               // K * 128 * 128 has to stay below 2^31
+    if ((st = check_queues(nq, queues)) != clblasSuccess) return st;
+    if ((st = check_events(nev, wait)) != clblasSuccess) return st;
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(queues[0]);
+    ResultDevice dev(C);
+    if (K != 0 && on_other_device(A, dev.device)) return clblasInvalidMatA;
+    if (K != 0 && on_other_device(B, dev.device)) return clblasInvalidMatB;
+    if (scaleA && (st = check_f32_vector(scaleA, offSA, M, dev.device, clblasInvalidVecX, clblasInsufficientMemVecX)) != clblasSuccess) return st;
+    if (scaleB && (st = check_f32_vector(scaleB, offSB, N, dev.device, clblasInvalidVecY, clblasInsufficientMemVecY)) != clblasSuccess) return st;
+    if ((st = wait_all(s, nev, wait)) != clblasSuccess) return st;
+
+    const signed char* a = static_cast<const signed char*>(A) + offA;
+    const signed char* b = static_cast<const signed char*>(B) + offB;
+    const float* sa = scaleA ? static_cast<const float*>(scaleA) + offSA : nullptr;
+    const float* sb = scaleB ? static_cast<const float*>(scaleB) + offSB : nullptr;
+    const bool ta = transA != clblasNoTrans, tb = transB != clblasNoTrans;
+    I8GemmProblem p = {};
+    p.K = K; p.alpha = alpha; p.beta = beta; p.type = type; p.C = C; p.offC = offC; p.ldc = ldc;
+    if (order == clblasRowMajor) {                         // lines of C are rows: row i of op(A) against column j of op(B)
+        p.lines = M; p.len = N;
+        p.P = a; p.ldp = lda; p.p_kcontig = !ta; p.s_lines = sa;
+        p.Q = b; p.ldq = ldb; p.q_kcontig = tb;  p.s_len = sb;
+    } else {
+        p.lines = N; p.len = M;
+        p.P = b; p.ldp = ldb; p.p_kcontig = !tb; p.s_lines = sb;
+        p.Q = a; p.ldq = lda; p.q_kcontig = ta;  p.s_len = sa;
+    }
+    const cudaError_t e = i8gemm(p, s);
+    if (e != cudaSuccess) { cudaGetLastError(); return from_cuda(e); }
+    return record_out(nq, queues, events);
+}
+
 }  // namespace
 
 void count_launch(unsigned n) { g_launches.fetch_add(n, std::memory_order_relaxed); }
@@ -1143,7 +1268,7 @@ unsigned long long clblasB200LaunchCount(void) { return g_launches.load(); }
 unsigned clblasB200DeviceFault(void)
 {
     if (cudaDeviceSynchronize() != cudaSuccess) { cudaGetLastError(); return 0x80000000u; }
-    return dgemm_tma_fault_flag() | sgemm_tma_fault_flag() | sgemm_3xtf32_fault_flag() | dtrsm_fused_fault_flag();
+    return dgemm_tma_fault_flag() | sgemm_tma_fault_flag() | sgemm_3xtf32_fault_flag() | dtrsm_fused_fault_flag() | i8gemm_fault_flag();
 }
 const char* clblasB200LastGemmKernel(void) { return t_last_kernel; }
 const char* clblasB200LastGemmVariant(void) { return t_last_variant; }
@@ -1188,6 +1313,23 @@ clblasStatus clblasB200DtrsmSharded(clblasOrder order, clblasSide side, clblasUp
 {
     return trsm_sharded_entry<double>(order, side, uplo, transA, diag, M, N, alpha, A, offA, lda, B, offB, ldb, comm, root,
                                       nq, queues, nev, wait, events);
+}
+
+clblasStatus clblasB200QuantizeI8(clblasOrder order, clblasSide side, size_t M, size_t N, clblasB200Type typeX, const clblasMem X, size_t offX,
+                                  size_t ldx, clblasMem Q, size_t offQ, size_t ldq, clblasMem scale, size_t offScale,
+                                  unsigned nq, clblasQueue* queues, unsigned nev, const clblasEvent* wait, clblasEvent* events)
+{
+    return quantize_entry(order, side, M, N, (int)typeX, X, offX, ldx, Q, offQ, ldq, scale, offScale, nq, queues, nev, wait, events);
+}
+
+clblasStatus clblasB200I8gemm(clblasOrder order, clblasTranspose transA, clblasTranspose transB, size_t M, size_t N, size_t K, float alpha,
+                              const clblasMem A, size_t offA, size_t lda, const clblasMem scaleA, size_t offScaleA,
+                              const clblasMem B, size_t offB, size_t ldb, const clblasMem scaleB, size_t offScaleB,
+                              float beta, clblasB200Type typeC, clblasMem C, size_t offC, size_t ldc,
+                              unsigned nq, clblasQueue* queues, unsigned nev, const clblasEvent* wait, clblasEvent* events)
+{
+    return i8gemm_entry(order, transA, transB, M, N, K, alpha, A, offA, lda, scaleA, offScaleA, B, offB, ldb, scaleB, offScaleB, beta,
+                        (int)typeC, C, offC, ldc, nq, queues, nev, wait, events);
 }
 int clblasB200SetGemmPath(int path) { return g_forced_path.exchange(path); }
 

@@ -288,6 +288,25 @@ cudaError_t launch_dtrsm_diag_fused(bool trans, bool forward, const double* A, s
 cudaError_t dtrsm_diag_fused_prepare_all();
 unsigned dtrsm_fused_fault_flag();
 
+// 8-bit product with scales (i8gemm.cu).  C is stored as `lines` lines of `len` contiguous elements (pitch ldc);
+// element (l, j) = alpha * s_lines[l] * s_len[j] * sum_k P[l, k] Q[j, k] + beta * C.  p_kcontig / q_kcontig: the operand is stored
+// with k contiguous (pitch ldp / ldq between values of l / j), else with l / j contiguous (pitch between values of k).
+// Null scales are ones.
+struct I8GemmProblem {
+    size_t lines, len, K;
+    float alpha, beta;
+    const signed char* P; size_t ldp; bool p_kcontig; const float* s_lines;
+    const signed char* Q; size_t ldq; bool q_kcontig; const float* s_len;
+    int type;                      // clblasB200Type of C
+    void* C; size_t offC, ldc;
+};
+cudaError_t i8gemm(const I8GemmProblem& p, cudaStream_t s);
+unsigned i8gemm_fault_flag();
+
+// 8-bit quantisation of `lines` lines of `len` contiguous elements, one scale per line or per position (quantize_i8.cu).
+cudaError_t quantize_i8(int type, bool per_line, const void* X, size_t offX, size_t ldx, signed char* Q, size_t ldq, float* scale,
+                        size_t lines, size_t len, cudaStream_t s);
+
 // Sticky per-translation-unit flags set when a bounded mbarrier wait inside a kernel ran out.
 unsigned dgemm_tma_fault_flag();
 unsigned sgemm_tma_fault_flag();

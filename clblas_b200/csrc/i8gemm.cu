@@ -1,0 +1,274 @@
+// C <- alpha * diag(sA) * op(A) * op(B) * diag(sB) + beta * C, A and B signed 8-bit integers, C in FP32, FP16 or BF16.
+// (No counterpart in the reference, whose products are FP32 / FP64: the linear layer of a language model with one scale per
+// token and per output channel.)
+//
+// The products are exact: tcgen05.mma.kind::i8 accumulates in 32-bit integers, |sum| <= K * 2^14 < 2^31 for the K <= 131071 the
+// front end admits, in any order and over any split of K.  The sum is rounded once to FP32, scaled in FP32 (three
+// roundings) and rounded once to the type of C.
+//
+// Both operands are read k-contiguous with 128-byte slabs (narrow_mma.cuh); an operand stored the other way, or not 16-byte
+// aligned, is transposed / copied once into a workspace.
+#include "narrow_mma.cuh"
+
+namespace cb200 {
+
+namespace {
+
+using namespace narrow;
+
+template <typename T> __device__ __forceinline__ float to_f(T v);
+template <> __device__ __forceinline__ float to_f(float v) { return v; }
+template <> __device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+template <> __device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> __device__ __forceinline__ T from_f(float v);
+template <> __device__ __forceinline__ float from_f(float v) { return v; }
+template <> __device__ __forceinline__ __half from_f(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f(float v) { return __float2bfloat16_rn(v); }
+
+template <typename T>
+struct EpiScaled {
+    static constexpr bool kMirror = false;
+    struct State {};
+    const float* su;                // scales of the rows u and the columns v; nullptr: ones
+    const float* sv;
+    float alpha, beta;
+    T* C;
+    size_t ld;
+    bool trans;                     // element (u, v) at C[v * ld + u] instead of C[u * ld + v]
+    bool vec_c, vec_s;              // 16-byte accesses of C and of sv allowed
+
+    __device__ bool transposed() const { return trans; }
+    __device__ float begin(State&, unsigned, unsigned u) const { return su ? alpha * su[u] : alpha; }
+    __device__ void column(State&, unsigned, unsigned u, unsigned v, float x) const
+    {
+        T* c = C + (size_t)v * ld + u;
+        float r = sv ? x * sv[v] : x;
+        if (beta != 0.f) r = fmaf(beta, to_f(*c), r);
+        *c = from_f<T>(r);
+    }
+    __device__ void segment(State&, unsigned, unsigned u, unsigned v, unsigned n, float (&x)[8]) const
+    {
+        T* c = C + (size_t)u * ld + v;
+        if (vec_c && n == 8) {
+            constexpr int W = 16 / sizeof(T);
+            float w[8];
+            if (sv && vec_s) {
+                *reinterpret_cast<float4*>(w) = __ldg(reinterpret_cast<const float4*>(sv + v));
+                *reinterpret_cast<float4*>(w + 4) = __ldg(reinterpret_cast<const float4*>(sv + v) + 1);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; i++) w[i] = sv ? __ldg(sv + v + i) : 1.f;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] *= w[i];
+#pragma unroll
+            for (int h = 0; h < 8 / W; h++) {
+                uint4 raw;
+                T* t = reinterpret_cast<T*>(&raw);
+                if (beta != 0.f) {
+                    raw = *(reinterpret_cast<const uint4*>(c) + h);
+#pragma unroll
+                    for (int i = 0; i < W; i++) x[h * W + i] = fmaf(beta, to_f(t[i]), x[h * W + i]);
+                }
+#pragma unroll
+                for (int i = 0; i < W; i++) t[i] = from_f<T>(x[h * W + i]);
+                *(reinterpret_cast<uint4*>(c) + h) = raw;
+            }
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            if (i >= (int)n) break;
+            float r = sv ? x[i] * __ldg(sv + v + i) : x[i];
+            if (beta != 0.f) r = fmaf(beta, to_f(c[i]), r);
+            c[i] = from_f<T>(r);
+        }
+    }
+    __device__ void end(State&, unsigned, unsigned) const {}
+};
+
+// C <- beta * C (K == 0 or alpha == 0): lines of `len` contiguous elements.
+template <typename T>
+__global__ void scale_lines_kernel(T* C, size_t lines, size_t len, size_t ld, float beta)
+{
+    const size_t total = lines * len;
+    for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (size_t)gridDim.x * blockDim.x) {
+        T* c = C + (i / len) * ld + i % len;
+        *c = from_f<T>(beta == 0.f ? 0.f : beta * to_f(*c));
+    }
+}
+
+// dst[r][k] (row pitch ldd, a multiple of 16) <- src[k][r] (pitch lds).  128 x 128 bytes per CTA: words of four r are read
+// along r, 4 x 4 bytes are exchanged in registers, words of four k go to shared memory (word w of row r at w ^ (r / 4), free of
+// bank conflicts both ways) and leave as 128-byte rows.
+template <bool WORDS>
+__global__ void __launch_bounds__(256) transpose_bytes_kernel(unsigned char* __restrict__ dst, size_t ldd, const unsigned char* __restrict__ src,
+                                                              size_t lds, size_t rows, size_t K)
+{
+    __shared__ uint32_t tile[128 * 32];
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const size_t r0 = (size_t)blockIdx.x * 128, k0 = (size_t)blockIdx.y * 128;
+    const size_t r = r0 + 4 * lane;
+#pragma unroll
+    for (int g = 0; g < 4; g++) {
+        const int kw = warp * 4 + g;                       // word of four k
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const size_t k = k0 + 4 * kw + i;
+            const unsigned char* p = src + k * lds + r;
+            w[i] = 0;
+            if (k < K) {
+                if (WORDS && r + 4 <= rows) {
+                    w[i] = *reinterpret_cast<const uint32_t*>(p);
+                } else {
+#pragma unroll
+                    for (int b = 0; b < 4; b++)
+                        if (r + b < rows) w[i] |= (uint32_t)p[b] << (8 * b);
+                }
+            }
+        }
+        const uint32_t a = __byte_perm(w[0], w[1], 0x5140), b = __byte_perm(w[2], w[3], 0x5140);      // bytes 0, 1 of each pair
+        const uint32_t c = __byte_perm(w[0], w[1], 0x7362), d = __byte_perm(w[2], w[3], 0x7362);      // bytes 2, 3
+        const uint32_t o[4] = {__byte_perm(a, b, 0x5410), __byte_perm(a, b, 0x7632), __byte_perm(c, d, 0x5410), __byte_perm(c, d, 0x7632)};
+#pragma unroll
+        for (int i = 0; i < 4; i++) tile[(4 * lane + i) * 32 + (kw ^ lane)] = o[i];
+    }
+    __syncthreads();
+    for (int i = warp; i < 128; i += 8) {
+        const size_t row = r0 + i, k = k0 + 4 * lane;
+        if (row < rows && k < K) *reinterpret_cast<uint32_t*>(dst + row * ldd + k) = tile[i * 32 + (lane ^ (i / 4))];      // ldd covers the last word
+    }
+}
+
+// dst[r][k] <- src[r][k] for a source of any alignment.  A word of dst is cut out of the two aligned source words that hold it
+// when both lie inside the row, and collected byte by byte at its ends.
+__global__ void __launch_bounds__(256) copy_bytes_kernel(unsigned char* __restrict__ dst, size_t ldd, const unsigned char* __restrict__ src,
+                                                         size_t lds, size_t rows, size_t K)
+{
+    const size_t words = (K + 3) / 4, total = rows * words;
+    for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (size_t)gridDim.x * blockDim.x) {
+        const size_t row = i / words, w = i % words;
+        const unsigned char* line = src + row * lds;
+        const unsigned char* p = line + 4 * w;
+        const unsigned mis = (unsigned)(reinterpret_cast<uintptr_t>(p) & 3u);
+        const unsigned char* q = p - mis;
+        uint32_t v = 0;
+        if (q >= line && q + (mis ? 8 : 4) <= line + K) {
+            const uint32_t lo = *reinterpret_cast<const uint32_t*>(q);
+            v = mis ? __funnelshift_r(lo, *reinterpret_cast<const uint32_t*>(q + 4), 8 * mis) : lo;
+        } else {
+#pragma unroll
+            for (int b = 0; b < 4; b++)
+                if (4 * w + b < K) v |= (uint32_t)p[b] << (8 * b);
+        }
+        *reinterpret_cast<uint32_t*>(dst + row * ldd + 4 * w) = v;
+    }
+}
+
+cudaError_t pack_operand(unsigned char* dst, size_t ldd, const void* src, size_t lds, size_t rows, size_t K, bool transpose, cudaStream_t s)
+{
+    const unsigned char* p = static_cast<const unsigned char*>(src);
+    if (transpose) {
+        const dim3 grid((unsigned)((rows + 127) / 128), (unsigned)((K + 127) / 128));
+        if (((reinterpret_cast<uintptr_t>(p) | lds) & 3u) == 0) transpose_bytes_kernel<true><<<grid, 256, 0, s>>>(dst, ldd, p, lds, rows, K);
+        else transpose_bytes_kernel<false><<<grid, 256, 0, s>>>(dst, ldd, p, lds, rows, K);
+    } else {
+        const size_t total = rows * ((K + 3) / 4), want = (total + 255) / 256, most = (size_t)sm_count() * 16;
+        copy_bytes_kernel<<<(unsigned)(want < most ? want : most), 256, 0, s>>>(dst, ldd, p, lds, rows, K);
+    }
+    count_launch();
+    return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t multiply(const Operand& lines, const Operand& len, const float* s_lines, const float* s_len, float alpha, float beta, T* C,
+                     size_t ldc, cudaStream_t st)
+{
+    // C is `lines.rows` lines of `len.rows` contiguous elements.
+    const size_t L = lines.rows, W = len.rows, K = lines.inner;
+    const bool vec_c = aligned16(C) && (ldc * sizeof(T)) % 16 == 0;
+    const unsigned nk = (unsigned)((K + slab_k(KIND_I8) - 1) / slab_k(KIND_I8));
+    const unsigned sms = (unsigned)sm_count();
+    Shape s = {};
+    s.K = (unsigned)K;
+    s.batch = 1;
+    auto normal = [&] {
+        s.U = (unsigned)L; s.V = (unsigned)W;
+        return EpiScaled<T>{s_lines, s_len, alpha, beta, C, ldc, false, vec_c, aligned16(s_len)};
+    };
+    auto split_for = [&](unsigned bn, unsigned per_sm) {
+        const size_t tiles = ((s.U + BM - 1) / BM) * (size_t)((s.V + bn - 1) / bn);
+        unsigned split = 1;
+        while (split < 8 && tiles * split * 2 <= (size_t)sms * per_sm && split * 2 * 2 <= nk) split *= 2;
+        return split;
+    };
+    if (L <= 128 && W > L) {
+        // Few lines (decoding): the contiguous dimension supplies the 128 rows of the instruction, the lines its columns.
+        s.U = (unsigned)W; s.V = (unsigned)L;
+        const EpiScaled<T> epi{s_len, s_lines, alpha, beta, C, ldc, true, false, false};
+        if (L <= 32) return run_split_by<KIND_I8, 32, false>(split_for(32, 2), len, lines, s, epi, st);
+        if (L <= 64) return run_split_by<KIND_I8, 64, false>(split_for(64, 2), len, lines, s, epi, st);
+        return run_split_by<KIND_I8, 128, false>(split_for(128, 1), len, lines, s, epi, st);
+    }
+    const EpiScaled<T> epi = normal();
+    if (W <= 32) return run_split_by<KIND_I8, 32, false>(split_for(32, 2), lines, len, s, epi, st);
+    if (W <= 64) return run_split_by<KIND_I8, 64, false>(split_for(64, 2), lines, len, s, epi, st);
+    const size_t tiles128 = ((L + 127) / 128) * ((W + 127) / 128);
+    if (tiles128 <= sms) return run_split_by<KIND_I8, 128, false>(split_for(128, 1), lines, len, s, epi, st);
+    return run_persistent<KIND_I8, 256, 2, false>(lines, len, s, epi, st);
+}
+
+template <typename T>
+cudaError_t i8gemm_typed(const I8GemmProblem& p, cudaStream_t s)
+{
+    T* C = static_cast<T*>(p.C) + p.offC;
+    if (p.K == 0 || p.alpha == 0.f) {
+        if (p.beta == 1.f) return cudaSuccess;
+        const size_t want = (p.lines * p.len + 255) / 256, most = (size_t)sm_count() * 16;
+        scale_lines_kernel<T><<<(unsigned)(want < most ? want : most), 256, 0, s>>>(C, p.lines, p.len, p.ldc, p.beta);
+        count_launch();
+        return cudaGetLastError();
+    }
+    if (p.lines >= (1u << 31) || p.len >= (1u << 31)) return cudaErrorNotSupported;
+    auto usable = [](const void* q, size_t ld, bool kcontig) { return kcontig && aligned16(q) && ld % 16 == 0; };
+    const bool fixP = !usable(p.P, p.ldp, p.p_kcontig), fixQ = !usable(p.Q, p.ldq, p.q_kcontig);
+    const size_t kld = (p.K + 15) / 16 * 16;
+    Operand a{p.P, p.K, p.lines, p.ldp, 0}, b{p.Q, p.K, p.len, p.ldq, 0};
+    unsigned char* ws = nullptr;
+    cudaError_t e = cudaSuccess;
+    if (fixP || fixQ) {
+        const size_t pn = fixP ? kld * p.lines : 0, qn = fixQ ? kld * p.len : 0, at = (pn + 255) / 256 * 256;
+        if ((e = ws_alloc(reinterpret_cast<void**>(&ws), at + qn, s)) != cudaSuccess) return e;
+        if (fixP) {
+            e = pack_operand(ws, kld, p.P, p.ldp, p.lines, p.K, !p.p_kcontig, s);
+            a.base = ws; a.ld = kld;
+        }
+        if (e == cudaSuccess && fixQ) {
+            e = pack_operand(ws + at, kld, p.Q, p.ldq, p.len, p.K, !p.q_kcontig, s);
+            b.base = ws + at; b.ld = kld;
+        }
+    }
+    if (e == cudaSuccess) e = multiply<T>(a, b, p.s_lines, p.s_len, p.alpha, p.beta, C, p.ldc, s);
+    if (ws) {
+        const cudaError_t e2 = ws_free(ws, s);
+        if (e == cudaSuccess) e = e2;
+    }
+    return e;
+}
+
+}  // namespace
+
+cudaError_t i8gemm(const I8GemmProblem& p, cudaStream_t s)
+{
+    set_last_kernel("i8gemm_tcgen05");
+    switch (p.type) {
+        case clblasB200Float32: return i8gemm_typed<float>(p, s);
+        case clblasB200Float16: return i8gemm_typed<__half>(p, s);
+        default: return i8gemm_typed<__nv_bfloat16>(p, s);
+    }
+}
+
+unsigned i8gemm_fault_flag() { return read_wait_timeout_flag(); }
+
+}  // namespace cb200

@@ -440,6 +440,39 @@ clblasStatus clblasB200DtrsmSharded(
  *      max_panels+1 entries).  Pure host arithmetic, exported for the tests. */
 clblasStatus clblasB200PanelPlan(size_t columns, size_t min_columns, unsigned max_panels, size_t* bounds, unsigned* count);
 
+/* ---- narrow types (no counterpart in the reference): the level-3 operators of a language model's linear layers ----------
+ *      Order, transposition, offsets (in elements), queues and events as in clblasSgemm; the work runs on
+ *      commandQueues[0], on the device that holds the result, whatever device is current; a buffer of another device or a
+ *      queue of another device is refused.  The buffers must not overlap unless said. */
+typedef enum clblasB200Type_ { clblasB200Float32 = 0, clblasB200Float16 = 1, clblasB200Bfloat16 = 2 } clblasB200Type;
+
+/*      X (M x N, FP32 / FP16 / BF16) in signed 8-bit integers with one FP32 scale per row (side = clblasLeft:
+ *      X ~ diag(scale) * Q) or per column (clblasRight: X ~ Q * diag(scale)):
+ *          scale = max|x| / 127,   q = rint(x * (127 / max|x|)),   each operation one IEEE FP32 operation, ties to even.
+ *      A row (column) of magnitudes below 2^-100 counts as zero: scale 0, q 0.  One that holds a NaN or an infinity gets
+ *      scale NaN and q 0, so that every product with it is NaN.
+ *      Checks: X (A's status codes), Q (B's), scale (clblasInvalidVecX, clblasInsufficientMemVecX). */
+clblasStatus clblasB200QuantizeI8(
+    clblasOrder order, clblasSide side, size_t M, size_t N,
+    clblasB200Type typeX, const clblasMem X, size_t offX, size_t ldx,
+    clblasMem Q, size_t offQ, size_t ldq,
+    clblasMem scale, size_t offScale,
+    unsigned numCommandQueues, clblasQueue* commandQueues,
+    unsigned numEventsInWaitList, const clblasEvent* eventWaitList, clblasEvent* events);
+
+/*      C <- alpha * diag(scaleA) * op(A) * op(B) * diag(scaleB) + beta * C, A and B signed 8-bit integers, C of typeC,
+ *      scaleA: M and scaleB: N FP32 values (NULL: ones).  op(A)*op(B) is exact (32-bit integers; K <= 131071, else
+ *      clblasInvalidDim); the scaling is FP32 and C is rounded once.  beta == 0 never reads C; alpha == 0 or K == 0
+ *      never reads A, B or the scales.
+ *      Checks: those of clblasSgemm in its order, then the scales (VecX for scaleA, VecY for scaleB). */
+clblasStatus clblasB200I8gemm(
+    clblasOrder order, clblasTranspose transA, clblasTranspose transB, size_t M, size_t N, size_t K, float alpha,
+    const clblasMem A, size_t offA, size_t lda, const clblasMem scaleA, size_t offScaleA,
+    const clblasMem B, size_t offB, size_t ldb, const clblasMem scaleB, size_t offScaleB,
+    float beta, clblasB200Type typeC, clblasMem C, size_t offC, size_t ldc,
+    unsigned numCommandQueues, clblasQueue* commandQueues,
+    unsigned numEventsInWaitList, const clblasEvent* eventWaitList, clblasEvent* events);
+
 /* ---- introspection used by the benchmark client and the tests (no reference counterpart
  *      beyond the AUTOGEMM_PRINT_DEBUG kernel-name print of xgemm.cc:437-445) ------------- */
 
