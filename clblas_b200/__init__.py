@@ -202,6 +202,9 @@ def _load() -> ctypes.CDLL:
     lib.clblasB200I8gemm.argtypes = [i, i, i, sz, sz, sz, ctypes.c_float, vp, sz, sz, vp, sz, vp, sz, sz, vp, sz,
                                      ctypes.c_float, i, vp, sz, sz] + tail
     lib.clblasB200I8gemm.restype = i
+    lib.clblasB200Orthogonalize.argtypes = [i, sz, sz, sz, u, ctypes.POINTER(ctypes.c_float), ctypes.c_float, i, vp, sz, sz, sz,
+                                            ctypes.c_float, vp, sz, sz, sz] + tail
+    lib.clblasB200Orthogonalize.restype = i
     return lib
 
 
@@ -215,7 +218,7 @@ EXPORTS = ["clblasSetup", "clblasTeardown", "clblasGetVersion", "clblasSgemm", "
     "clblasB200LastGemmVariant", "clblasB200WorkspaceAllocCount", "clblasB200NoAllocLimits", "clblasB200CommGetUniqueId",
     "clblasB200CommInitRank", "clblasB200CommInitAll", "clblasB200CommDestroy", "clblasB200CommInfo", "clblasB200PanelPlan",
     "clblasB200SgemmSharded", "clblasB200DgemmSharded", "clblasB200StrsmSharded", "clblasB200DtrsmSharded",
-    "clblasB200QuantizeI8", "clblasB200I8gemm"]
+    "clblasB200QuantizeI8", "clblasB200I8gemm", "clblasB200Orthogonalize"]
 
 
 def _ptr(x) -> Optional[int]:
@@ -307,6 +310,20 @@ def clblasB200I8gemm(order, transA, transB, M, N, K, alpha, A, offA, lda, scaleA
     nq, q, nw, w, e = _queues_events(queues, wait, events)
     return lib.clblasB200I8gemm(order, transA, transB, M, N, K, alpha, _ptr(A), offA, lda, _ptr(scaleA), offScaleA,
                                 _ptr(B), offB, ldb, _ptr(scaleB), offScaleB, beta, typeC, _ptr(C), offC, ldc, nq, q, nw, w, e)
+
+
+def clblasB200Orthogonalize(order, M, N, batchCount, steps, coefficients, alpha, typeG, G, offG, ldg, strideG, beta, O, offO, ldo,
+                            strideO, queues=None, wait=None, events=None) -> int:
+    """O <- alpha NS(G) + beta O, NS the Newton-Schulz orthogonalisation in ``steps`` steps, for ``batchCount`` matrices; O is
+    bfloat16.  ``coefficients``: ``None`` for (3.4445, -4.7750, 2.0315) in every step, or one (a, b, c) per step."""
+    if coefficients is not None:
+        flat = [float(x) for triple in coefficients for x in triple]
+        if len(flat) != 3 * steps:
+            raise ValueError("coefficients: one (a, b, c) for each step")
+        coefficients = (ctypes.c_float * len(flat))(*flat)
+    nq, q, nw, w, e = _queues_events(queues, wait, events)
+    return lib.clblasB200Orthogonalize(order, M, N, batchCount, steps, coefficients, alpha, typeG, _ptr(G), offG, ldg, strideG,
+                                       beta, _ptr(O), offO, ldo, strideO, nq, q, nw, w, e)
 
 
 def _host_addr(x) -> Optional[int]:

@@ -4,6 +4,7 @@
 #include "common.h"
 
 #include <atomic>
+#include <cmath>
 #include <cstdlib>
 #include <cstring>
 #include <mutex>
@@ -853,6 +854,51 @@ clblasStatus i8gemm_entry(clblasOrder order, clblasTranspose transA, clblasTrans
     return record_out(nq, queues, events);
 }
 
+// Extent of a batch of matrices beyond that of the first, which check_matrix_sizes has covered.
+clblasStatus check_batch_extent(size_t tsize, size_t lines, size_t len, const void* buf, size_t off, size_t ld, size_t batch, size_t stride,
+                                clblasStatus insufficient)
+{
+    size_t avail = 0;
+    if (batch > 1 && (!bytes_after(buf, &avail) || stride > avail / tsize / (batch - 1) ||
+                      off + (batch - 1) * stride + (lines - 1) * ld + len > avail / tsize))
+        return insufficient;
+    return clblasSuccess;
+}
+
+clblasStatus orthogonalize_entry(clblasOrder order, size_t M, size_t N, size_t batch, unsigned steps, const float* coeffs, float alpha,
+                                 int type, const void* G, size_t offG, size_t ldg, size_t strideG,
+                                 float beta, void* O, size_t offO, size_t ldo, size_t strideO,
+                                 unsigned nq, clblasQueue* queues, unsigned nev, const clblasEvent* wait, clblasEvent* events)
+{
+    if (G == nullptr) return clblasInvalidMatA;
+    if (O == nullptr) return clblasInvalidMatC;
+    if (order != clblasRowMajor && order != clblasColumnMajor) return clblasInvalidValue;
+    if (!valid_type(type) || steps < 1 || steps > 64) return clblasInvalidValue;
+    for (unsigned i = 0; coeffs != nullptr && i < 3 * steps; i++)
+        if (!std::isfinite(coeffs[i])) return clblasInvalidValue;
+    if (batch == 0) return clblasInvalidDim;
+    const size_t lines = order == clblasRowMajor ? M : N, len = order == clblasRowMajor ? N : M;
+    clblasStatus st;
+    if ((st = check_matrix_sizes(type_size(type), order, clblasNoTrans, M, N, G, offG, ldg, SET_A)) != clblasSuccess) return st;
+    if ((st = check_batch_extent(type_size(type), lines, len, G, offG, ldg, batch, strideG, clblasInsufficientMemMatA)) != clblasSuccess) return st;
+    if ((st = check_matrix_sizes(2, order, clblasNoTrans, M, N, O, offO, ldo, SET_C)) != clblasSuccess) return st;
+    if ((st = check_batch_extent(2, lines, len, O, offO, ldo, batch, strideO, clblasInsufficientMemMatC)) != clblasSuccess) return st;
+    // Matrices of O one behind the other, or side by side in the lines of one wide matrix.
+    if (batch > 1 && strideO < (lines - 1) * ldo + len && (strideO < len || (lines > 1 && (batch - 1) * strideO + len > ldo))) return clblasInvalidLeadDimC;
+    if ((st = check_queues(nq, queues)) != clblasSuccess) return st;
+    if ((st = check_events(nev, wait)) != clblasSuccess) return st;
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(queues[0]);
+    ResultDevice dev(O);
+    if (on_other_device(G, dev.device)) return clblasInvalidMatA;
+    if ((st = wait_all(s, nev, wait)) != clblasSuccess) return st;
+    OrthProblem p = {};
+    p.lines = lines; p.len = len; p.batch = batch; p.steps = (int)steps; p.coeffs = coeffs; p.alpha = alpha; p.beta = beta;
+    p.type = type; p.G = G; p.offG = offG; p.ldg = ldg; p.strideG = strideG; p.O = O; p.offO = offO; p.ldo = ldo; p.strideO = strideO;
+    const cudaError_t e = orthogonalize(p, s);
+    if (e != cudaSuccess) { cudaGetLastError(); return from_cuda(e); }
+    return record_out(nq, queues, events);
+}
+
 }  // namespace
 
 void count_launch(unsigned n) { g_launches.fetch_add(n, std::memory_order_relaxed); }
@@ -1268,7 +1314,8 @@ unsigned long long clblasB200LaunchCount(void) { return g_launches.load(); }
 unsigned clblasB200DeviceFault(void)
 {
     if (cudaDeviceSynchronize() != cudaSuccess) { cudaGetLastError(); return 0x80000000u; }
-    return dgemm_tma_fault_flag() | sgemm_tma_fault_flag() | sgemm_3xtf32_fault_flag() | dtrsm_fused_fault_flag() | i8gemm_fault_flag();
+    return dgemm_tma_fault_flag() | sgemm_tma_fault_flag() | sgemm_3xtf32_fault_flag() | dtrsm_fused_fault_flag() | i8gemm_fault_flag() |
+           orthogonalize_fault_flag();
 }
 const char* clblasB200LastGemmKernel(void) { return t_last_kernel; }
 const char* clblasB200LastGemmVariant(void) { return t_last_variant; }
@@ -1330,6 +1377,15 @@ clblasStatus clblasB200I8gemm(clblasOrder order, clblasTranspose transA, clblasT
 {
     return i8gemm_entry(order, transA, transB, M, N, K, alpha, A, offA, lda, scaleA, offScaleA, B, offB, ldb, scaleB, offScaleB, beta,
                         (int)typeC, C, offC, ldc, nq, queues, nev, wait, events);
+}
+
+clblasStatus clblasB200Orthogonalize(clblasOrder order, size_t M, size_t N, size_t batchCount, unsigned steps, const float* coefficients, float alpha,
+                                     clblasB200Type typeG, const clblasMem G, size_t offG, size_t ldg, size_t strideG,
+                                     float beta, clblasMem O, size_t offO, size_t ldo, size_t strideO,
+                                     unsigned nq, clblasQueue* queues, unsigned nev, const clblasEvent* wait, clblasEvent* events)
+{
+    return orthogonalize_entry(order, M, N, batchCount, steps, coefficients, alpha, (int)typeG, G, offG, ldg, strideG, beta, O, offO, ldo, strideO,
+                               nq, queues, nev, wait, events);
 }
 int clblasB200SetGemmPath(int path) { return g_forced_path.exchange(path); }
 

@@ -307,6 +307,19 @@ unsigned i8gemm_fault_flag();
 cudaError_t quantize_i8(int type, bool per_line, const void* X, size_t offX, size_t ldx, signed char* Q, size_t ldq, float* scale,
                         size_t lines, size_t len, cudaStream_t s);
 
+// Newton-Schulz orthogonalisation of `batch` matrices of `lines` lines of `len` contiguous elements (orthogonalize.cu).
+struct OrthProblem {
+    size_t lines, len, batch;
+    int steps;
+    const float* coeffs;           // 3 per step, host memory; null: the default triple in every step
+    float alpha, beta;
+    int type;                      // clblasB200Type of G
+    const void* G; size_t offG, ldg, strideG;
+    void* O; size_t offO, ldo, strideO;        // BF16
+};
+cudaError_t orthogonalize(const OrthProblem& p, cudaStream_t s);
+unsigned orthogonalize_fault_flag();
+
 // Sticky per-translation-unit flags set when a bounded mbarrier wait inside a kernel ran out.
 unsigned dgemm_tma_fault_flag();
 unsigned sgemm_tma_fault_flag();

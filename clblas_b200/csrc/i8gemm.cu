@@ -39,6 +39,7 @@ struct EpiScaled {
 
     __device__ bool transposed() const { return trans; }
     __device__ float begin(State&, unsigned, unsigned u) const { return su ? alpha * su[u] : alpha; }
+    template <int CH> __device__ void combine(State&, unsigned, unsigned, unsigned, unsigned, float (&)[CH]) const {}
     __device__ void column(State&, unsigned, unsigned u, unsigned v, float x) const
     {
         T* c = C + (size_t)v * ld + u;
@@ -214,9 +215,7 @@ cudaError_t multiply(const Operand& lines, const Operand& len, const float* s_li
     const EpiScaled<T> epi = normal();
     if (W <= 32) return run_split_by<KIND_I8, 32, false>(split_for(32, 2), lines, len, s, epi, st);
     if (W <= 64) return run_split_by<KIND_I8, 64, false>(split_for(64, 2), lines, len, s, epi, st);
-    const size_t tiles128 = ((L + 127) / 128) * ((W + 127) / 128);
-    if (tiles128 <= sms) return run_split_by<KIND_I8, 128, false>(split_for(128, 1), lines, len, s, epi, st);
-    return run_persistent<KIND_I8, 256, 2, false>(lines, len, s, epi, st);
+    return run_planned<KIND_I8, false>(lines, len, s, epi, st);
 }
 
 template <typename T>

@@ -208,6 +208,7 @@ __host__ __device__ inline void tile_coords(const Shape& s, unsigned t, unsigned
 //   epi.begin()    per thread and tile; returns the factor of this lane's row, applied to the accumulator
 //   epi.column()   one value per lane, u contiguous over the lanes: transposed results and mirrored tiles
 //   epi.segment()  up to 8 values with consecutive v of one row
+//   epi.combine()  transposed results only: what the row contributes besides the accumulator, before column()
 // ---------------------------------------------------------------------------------------------------------------------
 
 template <class Epi, int CH>
@@ -218,9 +219,13 @@ __device__ __forceinline__ void epilogue_chunk(const Epi& epi, typename Epi::Sta
     if (epi.transposed() || (Epi::kMirror && mirror)) {
         const unsigned u = u0 + lane;
         if (u < s.U) {
+            float y[CH];
+#pragma unroll
+            for (int j = 0; j < CH; j++) y[j] = x[j];
+            if (epi.transposed()) epi.template combine<CH>(st, z, u, v0, s.V, y);
 #pragma unroll
             for (int j = 0; j < CH; j++)
-                if (v0 + j < s.V) epi.column(st, z, u, v0 + j, x[j]);
+                if (v0 + j < s.V) epi.column(st, z, u, v0 + j, y[j]);
         }
         if (epi.transposed()) return;
     }
@@ -654,6 +659,30 @@ cudaError_t run_split(const Operand& p, const Operand& q, Shape s, const Epi& ep
     return launch(kernel, s.tiles * s.batch * S, S, smem, st, mp, mq, s, epi);
 }
 
+// How a product of more than 64 columns runs.  Estimated clocks: rounds of tiles times (slabs x clocks per slab + what a tile costs besides).
+//   pairs:  256 x 256 tiles on pairs of CTAs, 512 clocks per slab
+//   single: 128 x 128 tiles, persistent, 300 clocks per slab (both operands are read from shared memory at its full rate)
+//   split:  128 x 128 tiles, k over S CTAs of a cluster
+struct Plan { bool pairs; unsigned split; };         // split == 0: persistent
+inline Plan choose_plan(unsigned U, unsigned V, unsigned K, unsigned batch, int tri, int kind)
+{
+    const double sms = sm_count(), nk = (K + slab_k(kind) - 1) / slab_k(kind);
+    auto tiles = [&](unsigned b) {
+        const double tu = (U + b - 1) / b, tv = (V + b - 1) / b;
+        return batch * (tri ? tu * (tu + 1) / 2 : tu * tv);
+    };
+    auto rounds = [](double work, double slots) { const double r = work / slots; return (double)(unsigned long long)r + (r > (double)(unsigned long long)r); };
+    Plan best{true, 0};
+    double least = rounds(tiles(256), (double)((int)sms / 2)) * (nk * 512 + 500) + 4000;
+    const double t128 = tiles(128), single = rounds(t128, sms) * (nk * 300 + 500) + 3000;
+    if (single < least) { least = single; best = {false, 0}; }
+    for (unsigned s = 1; s <= 8 && s <= nk; s *= 2) {
+        const double c = rounds(t128 * s, sms) * ((double)(((unsigned)nk + s - 1) / s) * 300 + 3000 + (s > 1 ? 1500 : 0));
+        if (c < least) { least = c; best = {false, s}; }
+    }
+    return best;
+}
+
 template <int KIND, int BN, bool QMN, class Epi>
 cudaError_t run_split_by(unsigned split, const Operand& p, const Operand& q, const Shape& s, const Epi& epi, cudaStream_t st)
 {
@@ -663,6 +692,15 @@ cudaError_t run_split_by(unsigned split, const Operand& p, const Operand& q, con
         case 2: return run_split<KIND, BN, 2, QMN, Epi>(p, q, s, epi, st);
         default: return run_split<KIND, BN, 1, QMN, Epi>(p, q, s, epi, st);
     }
+}
+
+template <int KIND, bool QMN, class Epi>
+cudaError_t run_planned(const Operand& p, const Operand& q, const Shape& s, const Epi& epi, cudaStream_t st)
+{
+    const Plan plan = choose_plan(s.U, s.V, s.K, s.batch, s.tri, KIND);
+    if (plan.pairs) return run_persistent<KIND, 256, 2, QMN, Epi>(p, q, s, epi, st);
+    if (plan.split == 0) return run_persistent<KIND, 128, 1, QMN, Epi>(p, q, s, epi, st);
+    return run_split_by<KIND, 128, QMN, Epi>(plan.split, p, q, s, epi, st);
 }
 
 }  // namespace narrow

@@ -473,6 +473,25 @@ clblasStatus clblasB200I8gemm(
     unsigned numCommandQueues, clblasQueue* commandQueues,
     unsigned numEventsInWaitList, const clblasEvent* eventWaitList, clblasEvent* events);
 
+/*      O <- alpha * NS(G) + beta * O for batchCount matrices (M x N each, matrix i at off + i*stride): the Newton-Schulz
+ *      orthogonalisation of an update.  NS(G) = X_steps with X_0 = G / (|G|_F + 1e-7) and
+ *          X <- a X + b (X X') X + c (X X')^2 X
+ *      with (a, b, c) = coefficients[3k .. 3k+2] (host memory) in step k, or (3.4445, -4.7750, 2.0315) in every step when
+ *      coefficients is NULL.  1 <= steps <= 64.
+ *      G: FP32 / FP16 / BF16.  O: BF16 (the products take 11-bit operands: the result is good to about 1e-3 relative to
+ *      its own norm).  beta == 0 never reads O.  A G that holds a NaN or an infinity gives NaN everywhere.  The iteration
+ *      runs in FP16 with scale factors that leave room for singular values of X up to 16 and for |b| s^2 + |c| s^4 up to 255
+ *      at singular values s; coefficients that drive X further overflow.
+ *      G and O may be the same buffer, and matrices of G may overlap; matrices of O may not.
+ *      Workspace (from the library's pool): about 6 bytes per element of G and 4 per element of the smaller square.
+ *      Checks: G (A's status codes), O (C's; clblasInvalidLeadDimC also for a stride that makes its matrices overlap). */
+clblasStatus clblasB200Orthogonalize(
+    clblasOrder order, size_t M, size_t N, size_t batchCount, unsigned steps, const float* coefficients, float alpha,
+    clblasB200Type typeG, const clblasMem G, size_t offG, size_t ldg, size_t strideG,
+    float beta, clblasMem O, size_t offO, size_t ldo, size_t strideO,
+    unsigned numCommandQueues, clblasQueue* commandQueues,
+    unsigned numEventsInWaitList, const clblasEvent* eventWaitList, clblasEvent* events);
+
 /* ---- introspection used by the benchmark client and the tests (no reference counterpart
  *      beyond the AUTOGEMM_PRINT_DEBUG kernel-name print of xgemm.cc:437-445) ------------- */
 

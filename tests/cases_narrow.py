@@ -72,3 +72,68 @@ def quantize_reference(x, axis):
     scale = torch.where(live, top / full, torch.zeros_like(top))
     inv = torch.where(live, full / torch.where(live, top, full), torch.zeros_like(top))
     return (x * inv).round().to(torch.int8), scale.reshape(-1)
+
+
+QUINTIC = (3.4445, -4.7750, 2.0315)
+
+
+def orth_exact(g, coefficients):
+    """NS(G) of the definition in 64 bits; g: rows x cols, float64."""
+    x = g / (torch.linalg.matrix_norm(g) + 1e-7)
+    for a, b, c in coefficients:
+        q = x @ x.t() if x.shape[0] <= x.shape[1] else x.t() @ x
+        p = a * torch.eye(q.shape[0], dtype=torch.float64, device=q.device) + b * q + c * (q @ q)
+        x = p @ x if x.shape[0] <= x.shape[1] else x @ p
+    return x
+
+
+def orth_bound(g, coefficients):
+    """First-order bound of |computed - exact|_F before the rounding to BF16, from the roundings the operator makes.
+
+    In every step: the operands X, A = X X' - t I and P = (b + 2 c t) A + c A^2 are rounded to FP16 (u = 2^-11), X is kept in
+    two FP16 numbers (2^-22), sums are FP32.  An error E of X after step k, in the basis of the singular vectors, reaches the
+    result multiplied entry by entry by divided differences of the remaining polynomial F: (F_i - F_j) / (s_i - s_j) or
+    (F_i + F_j) / (s_i + s_j).  A rounding of A or P is met by X, so its column j carries s_j; the rounding of the
+    operand X is met by P, so its row i carries p_i; the rounding of the pair carries nothing."""
+    u = 2.0 ** -11
+    s = torch.linalg.svdvals(g.cpu().double())
+    n, m = s.numel(), max(g.shape)
+    s = s / (s.norm() + 1e-7)
+    chain = [s]
+    for a, b, c in coefficients:
+        s = s * (a + b * s ** 2 + c * s ** 4)
+        chain.append(s)
+    last = chain[-1]
+
+    def weights(k):
+        """Largest factor with which an entry (i, j) of an error of X after step k reaches the result: n x n."""
+        z = chain[k + 1]
+        if k + 1 == len(coefficients):
+            return torch.ones(n, n, dtype=torch.float64)
+        d = z[:, None] - z[None, :]
+        slope = torch.ones(n, dtype=torch.float64)
+        y = z
+        for a, b, c in coefficients[k + 1:]:
+            slope = slope * (a + 3 * b * y ** 2 + 5 * c * y ** 4)
+            y = y * (a + b * y ** 2 + c * y ** 4)
+        minus = torch.where(d.abs() > 1e-6, (last[:, None] - last[None, :]) / torch.where(d.abs() > 1e-6, d, torch.ones_like(d)),
+                            torch.maximum(slope.abs()[:, None], slope.abs()[None, :]))
+        t = z[:, None] + z[None, :]
+        plus = torch.where(t.abs() > 1e-12, (last[:, None] + last[None, :]) / torch.where(t.abs() > 1e-12, t, torch.ones_like(t)), slope.abs()[:, None])
+        return torch.maximum(minus.abs(), plus.abs())
+
+    total = 0.0
+    for k, (a, b, c) in enumerate(coefficients):
+        s = chain[k]
+        w = weights(k)
+        t = float((s ** 2).mean())
+        t = t if t >= 0.2 else 0.0
+        A = s ** 2 - t
+        P = (b + 2 * c * t) * A + c * A ** 2
+        # FP32 sums of tensor-core products, K / 16 of them, each within 2^-22 of the magnitudes (in norm at most |X|^2 and |A|^2, n-fold)
+        dA = u * float(A.norm()) + (m / 16 + 1) * 2.0 ** -22 * float(s.norm()) ** 2
+        dP = abs(b + 2 * c * t) * dA + 2 * abs(c) * float(A.abs().max()) * dA + u * float(P.norm()) + (n / 16 + 1) * 2.0 ** -22 * abs(c) * float(A.norm()) ** 2
+        total += dP * float((w * s[None, :]).max())
+        total += u * float(s.norm()) * float((w * P.abs()[:, None]).max())
+        total += ((n / 16 + 1) * 2.0 ** -22 * float(P.norm()) + 2.0 ** -21 * (abs(a) + 1)) * float(s.norm()) * float(w.max())
+    return total * 1.05                                     # the second order
