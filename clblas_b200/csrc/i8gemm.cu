@@ -25,66 +25,106 @@ template <> __device__ __forceinline__ float from_f(float v) { return v; }
 template <> __device__ __forceinline__ __half from_f(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f(float v) { return __float2bfloat16_rn(v); }
 
+template <typename T> __device__ __forceinline__ uint32_t pack16(float a, float b);
+template <> __device__ __forceinline__ uint32_t pack16<__half>(float a, float b) { const __half2 h = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t*>(&h); }
+template <> __device__ __forceinline__ uint32_t pack16<__nv_bfloat16>(float a, float b) { const __nv_bfloat162 h = __floats2bfloat162_rn(a, b); return *reinterpret_cast<const uint32_t*>(&h); }
+template <typename T> __device__ __forceinline__ float2 unpack16(uint32_t h);
+template <> __device__ __forceinline__ float2 unpack16<__half>(uint32_t h) { return __half22float2(*reinterpret_cast<const __half2*>(&h)); }
+template <> __device__ __forceinline__ float2 unpack16<__nv_bfloat16>(uint32_t h) { return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&h)); }
+
+// C[u, v] <- alpha su[u] sv[v] acc + beta C[u, v].
 template <typename T>
 struct EpiScaled {
-    static constexpr bool kMirror = false;
-    struct State {};
+    static constexpr bool kChained = false;
+    struct State { float factor[4]; };
+    template <int G> struct Pre { Bits16<G> c; };
     const float* su;                // scales of the rows u and the columns v; nullptr: ones
     const float* sv;
     float alpha, beta;
     T* C;
     size_t ld;
     bool trans;                     // element (u, v) at C[v * ld + u] instead of C[u * ld + v]
-    bool vec_c, vec_s;              // 16-byte accesses of C and of sv allowed
+    bool vec;                       // 16-byte accesses of C allowed
 
-    __device__ bool transposed() const { return trans; }
-    __device__ float begin(State&, unsigned, unsigned u) const { return su ? alpha * su[u] : alpha; }
-    template <int CH> __device__ void combine(State&, unsigned, unsigned, unsigned, unsigned, float (&)[CH]) const {}
-    __device__ void column(State&, unsigned, unsigned u, unsigned v, float x) const
+    __device__ void begin(State& st, const Shape& s, unsigned, unsigned u0) const
     {
-        T* c = C + (size_t)v * ld + u;
-        float r = sv ? x * sv[v] : x;
-        if (beta != 0.f) r = fmaf(beta, to_f(*c), r);
-        *c = from_f<T>(r);
+        const unsigned u = u0 + (threadIdx.x & 31) / 4;
+#pragma unroll
+        for (int g = 0; g < 4; g++) st.factor[g] = su && u + 8 * g < s.U ? alpha * __ldg(su + u + 8 * g) : alpha;
     }
-    __device__ void segment(State&, unsigned, unsigned u, unsigned v, unsigned n, float (&x)[8]) const
+    template <int G>
+    __device__ void fetch(Pre<G>& p, const Shape& s, unsigned, unsigned u0, unsigned v0) const
     {
-        T* c = C + (size_t)u * ld + v;
-        if (vec_c && n == 8) {
-            constexpr int W = 16 / sizeof(T);
-            float w[8];
-            if (sv && vec_s) {
-                *reinterpret_cast<float4*>(w) = __ldg(reinterpret_cast<const float4*>(sv + v));
-                *reinterpret_cast<float4*>(w + 4) = __ldg(reinterpret_cast<const float4*>(sv + v) + 1);
-            } else {
+        if (sizeof(T) == 2 && beta != 0.f && !trans) load_rows16<G>(p.c, reinterpret_cast<const uint16_t*>(C), ld, u0, v0, s.U, s.V, vec);
+    }
+    template <int G>
+    __device__ void chunk(State& st, Pre<G>& p, const Shape& s, unsigned z, unsigned u0, unsigned v0, unsigned v_next, bool, float (&x)[4][G][2]) const
+    {
+        const int lane = threadIdx.x & 31, q = lane & 3;
+        const unsigned u = u0 + lane / 4;
 #pragma unroll
-                for (int i = 0; i < 8; i++) w[i] = sv ? __ldg(sv + v + i) : 1.f;
+        for (int k = 0; k < G; k++) {
+            const unsigned v = v0 + 8 * k + 2 * q;
+            const float w0 = sv && v < s.V ? __ldg(sv + v) : 1.f, w1 = sv && v + 1 < s.V ? __ldg(sv + v + 1) : 1.f;
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                x[g][k][0] = x[g][k][0] * st.factor[g] * w0;
+                x[g][k][1] = x[g][k][1] * st.factor[g] * w1;
             }
+        }
+        if (beta != 0.f && (trans || sizeof(T) == 4)) {             // C in fragments
+            T old[4][G][2];
 #pragma unroll
-            for (int i = 0; i < 8; i++) x[i] *= w[i];
+            for (int g = 0; g < 4; g++)
 #pragma unroll
-            for (int h = 0; h < 8 / W; h++) {
-                uint4 raw;
-                T* t = reinterpret_cast<T*>(&raw);
-                if (beta != 0.f) {
-                    raw = *(reinterpret_cast<const uint4*>(c) + h);
+                for (int k = 0; k < G; k++)
 #pragma unroll
-                    for (int i = 0; i < W; i++) x[h * W + i] = fmaf(beta, to_f(t[i]), x[h * W + i]);
+                    for (int e = 0; e < 2; e++)
+                        if (u + 8 * g < s.U && v0 + 8 * k + 2 * q + e < s.V) old[g][k][e] = C[at(u + 8 * g, v0 + 8 * k + 2 * q + e)];
+#pragma unroll
+            for (int g = 0; g < 4; g++)
+#pragma unroll
+                for (int k = 0; k < G; k++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) x[g][k][e] = fmaf(beta, to_f(old[g][k][e]), x[g][k][e]);
+        }
+        if constexpr (sizeof(T) == 2) {
+            if (beta != 0.f && !trans) {
+                rows_to_fragments<G>(p.c, v0, s.V, vec);
+#pragma unroll
+                for (int g = 0; g < 4; g++)
+#pragma unroll
+                    for (int k = 0; k < G; k++) {
+                        const float2 c = unpack16<T>(p.c.h[g][k]);
+                        x[g][k][0] = fmaf(beta, c.x, x[g][k][0]);
+                        x[g][k][1] = fmaf(beta, c.y, x[g][k][1]);
+                    }
+            }
+            if (v_next != ~0u) fetch<G>(p, s, z, u0, v_next);
+            Bits16<G> o;
+#pragma unroll
+            for (int g = 0; g < 4; g++)
+#pragma unroll
+                for (int k = 0; k < G; k++) o.h[g][k] = pack16<T>(x[g][k][0], x[g][k][1]);
+            if (trans) store_columns16<G>(o, reinterpret_cast<uint16_t*>(C), ld, u0, v0, s.U, s.V, vec);
+            else store_rows16<G>(o, reinterpret_cast<uint16_t*>(C), ld, u0, v0, s.U, s.V, vec);
+        } else {                                                    // 32-bit: a quad's fragments fill 32 bytes of a row, eight lanes' 32 bytes of a column
+#pragma unroll
+            for (int g = 0; g < 4; g++)
+#pragma unroll
+                for (int k = 0; k < G; k++) {
+                    const unsigned v = v0 + 8 * k + 2 * q;
+                    if (u + 8 * g >= s.U) continue;
+                    float* c = reinterpret_cast<float*>(C) + at(u + 8 * g, v);
+                    if (!trans && vec && v + 2 <= s.V) *reinterpret_cast<float2*>(c) = make_float2(x[g][k][0], x[g][k][1]);
+                    else {
+                        if (v < s.V) *c = x[g][k][0];
+                        if (v + 1 < s.V) c[trans ? ld : 1] = x[g][k][1];
+                    }
                 }
-#pragma unroll
-                for (int i = 0; i < W; i++) t[i] = from_f<T>(x[h * W + i]);
-                *(reinterpret_cast<uint4*>(c) + h) = raw;
-            }
-            return;
-        }
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            if (i >= (int)n) break;
-            float r = sv ? x[i] * __ldg(sv + v + i) : x[i];
-            if (beta != 0.f) r = fmaf(beta, to_f(c[i]), r);
-            c[i] = from_f<T>(r);
         }
     }
+    __device__ size_t at(unsigned u, unsigned v) const { return trans ? (size_t)v * ld + u : (size_t)u * ld + v; }
     __device__ void end(State&, unsigned, unsigned) const {}
 };
 
@@ -196,7 +236,7 @@ cudaError_t multiply(const Operand& lines, const Operand& len, const float* s_li
     s.batch = 1;
     auto normal = [&] {
         s.U = (unsigned)L; s.V = (unsigned)W;
-        return EpiScaled<T>{s_lines, s_len, alpha, beta, C, ldc, false, vec_c, aligned16(s_len)};
+        return EpiScaled<T>{s_lines, s_len, alpha, beta, C, ldc, false, vec_c};
     };
     auto split_for = [&](unsigned bn, unsigned per_sm) {
         const size_t tiles = ((s.U + BM - 1) / BM) * (size_t)((s.V + bn - 1) / bn);
@@ -207,7 +247,7 @@ cudaError_t multiply(const Operand& lines, const Operand& len, const float* s_li
     if (L <= 128 && W > L) {
         // Few lines (decoding): the contiguous dimension supplies the 128 rows of the instruction, the lines its columns.
         s.U = (unsigned)W; s.V = (unsigned)L;
-        const EpiScaled<T> epi{s_len, s_lines, alpha, beta, C, ldc, true, false, false};
+        const EpiScaled<T> epi{s_len, s_lines, alpha, beta, C, ldc, true, vec_c};
         if (L <= 32) return run_split_by<KIND_I8, 32, false>(split_for(32, 2), len, lines, s, epi, st);
         if (L <= 64) return run_split_by<KIND_I8, 64, false>(split_for(64, 2), len, lines, s, epi, st);
         return run_split_by<KIND_I8, 128, false>(split_for(128, 1), len, lines, s, epi, st);

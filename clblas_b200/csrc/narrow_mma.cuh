@@ -20,6 +20,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <cmath>
+
 namespace cb200 {
 namespace narrow {
 
@@ -29,7 +31,6 @@ constexpr int BM = 128;                       // rows of P per CTA = lanes of te
 constexpr int SLAB_BYTES = 128;               // bytes along k per slab: one SWIZZLE_128B row
 constexpr int EPI_WARPS = 8;
 constexpr int THREADS = (2 + EPI_WARPS) * 32;
-constexpr int STAGE_BUF = 32 * 32 * 4;        // per epilogue warp: 32 x 32 values on their way to coalesced stores
 
 __host__ __device__ constexpr int slab_k(int kind) { return kind == KIND_I8 ? SLAB_BYTES : SLAB_BYTES / 2; }
 
@@ -62,9 +63,9 @@ __device__ __forceinline__ uint32_t map_shared(uint32_t saddr, uint32_t rank)
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(saddr), "r"(rank));
     return r;
 }
-__device__ __forceinline__ void st_cluster(uint32_t addr, uint32_t v)
+__device__ __forceinline__ void st_cluster(uint32_t addr, uint32_t v, uint32_t w)
 {
-    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+    asm volatile("st.shared::cluster.v2.u32 [%0], {%1, %2};" ::"r"(addr), "r"(v), "r"(w) : "memory");
 }
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t addr)
 {
@@ -154,21 +155,19 @@ __device__ __forceinline__ void tmem_free(uint32_t base, uint32_t cols)
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-// 32 consecutive 32-bit columns of this thread's tensor-memory lane, waited for.
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32])
+// 16 rows x 32 columns of 32-bit accumulators as the fragments of 8 x 8 blocks: lane t holds, for column group k, row t / 4 columns
+// 8 k + 2 (t % 4) + {0, 1} in v[4 k + {0, 1}] and row t / 4 + 8 of the same columns in v[4 k + {2, 3}].  The warp has to be converged.
+__device__ __forceinline__ void tmem_ld_16x32(uint32_t taddr, uint32_t (&v)[16])
 {
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
         : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
-          "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
-          "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
-          "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+          "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
         : "r"(taddr)
         : "memory");
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
+__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
 template <int KIND>
 __device__ __forceinline__ float acc_value(uint32_t v) { return KIND == KIND_I8 ? (float)(int)v : __uint_as_float(v); }
@@ -203,61 +202,135 @@ __host__ __device__ inline void tile_coords(const Shape& s, unsigned t, unsigned
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// Epilogue of 32 rows (one per lane) x CH columns held as x[CH] per lane.
-//   Epi::kMirror   also stores every value at (v, u) (symmetric results; tiles off the diagonal only)
-//   epi.begin()    per thread and tile; returns the factor of this lane's row, applied to the accumulator
-//   epi.column()   one value per lane, u contiguous over the lanes: transposed results and mirrored tiles
-//   epi.segment()  up to 8 values with consecutive v of one row
-//   epi.combine()  transposed results only: what the row contributes besides the accumulator, before column()
+// Epilogue.  A warp finishes chunks of 32 rows x 8 G columns, held as fragments x[g][k][e]: row 8 g + lane / 4, column
+// 8 k + 2 (lane % 4) + e.  What a functor has:
+//   kChained      launched as a link of a chain of products (programmatic dependent launch)
+//   begin()       per thread and tile
+//   Pre, fetch()  what a chunk needs besides the accumulators, requested one chunk ahead
+//   chunk()       computes and stores; requests the next chunk's (at column v_next, ~0u: none) as soon as its own is used; mirror: the
+//                 result is symmetric and the tile off its diagonal, so it is stored at (v, u) too
+//   end()         per thread and tile
+//
+// Nothing goes through shared memory: its bandwidth is what the products and the loads that feed them use up (both sides
+// together 128 bytes per clock), and an epilogue that staged its chunks there ran at a fifth of its speed beside them.
+// Rows are put together by exchanges among the four lanes that share one (quad_transpose), columns by transposing 8 x 8 blocks
+// (movmatrix); 16-bit results leave as 16 bytes a lane, 64 bytes a row.
 // ---------------------------------------------------------------------------------------------------------------------
 
-template <class Epi, int CH>
-__device__ __forceinline__ void epilogue_chunk(const Epi& epi, typename Epi::State& st, const Shape& s, float* buf, unsigned z, unsigned u0,
-                                               unsigned v0, bool mirror, const float (&x)[CH])
+// r[k] of lane j of a quad becomes r[j] of lane k.
+__device__ __forceinline__ void quad_transpose(uint32_t (&r)[4])
 {
-    const int lane = threadIdx.x & 31;
-    if (epi.transposed() || (Epi::kMirror && mirror)) {
-        const unsigned u = u0 + lane;
-        if (u < s.U) {
-            float y[CH];
+    const bool o1 = threadIdx.x & 1, o2 = threadIdx.x & 2;
+    uint32_t a = __shfl_xor_sync(0xffffffffu, o1 ? r[0] : r[1], 1), b = __shfl_xor_sync(0xffffffffu, o1 ? r[2] : r[3], 1);
+    if (o1) { r[0] = a; r[2] = b; } else { r[1] = a; r[3] = b; }
+    a = __shfl_xor_sync(0xffffffffu, o2 ? r[0] : r[2], 2);
+    b = __shfl_xor_sync(0xffffffffu, o2 ? r[1] : r[3], 2);
+    if (o2) { r[0] = a; r[1] = b; } else { r[2] = a; r[3] = b; }
+}
+// Transposes an 8 x 8 block of 16-bit values held as fragments.
+__device__ __forceinline__ uint32_t block_transpose(uint32_t v)
+{
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+
+// 16-bit matrices (as raw bits): a lane's share of a chunk, by rows (16 bytes per 8 rows) or by fragments.
+// `vec`: base and pitch allow 16-byte accesses; without it, and for chunks narrower than 32 columns, fragments are accessed directly.
+template <int G>
+struct Bits16 {
+    uint32_t h[4][G];                                       // [g][k]: two values of row 8 g + lane / 4, columns 8 k + 2 (lane % 4)
+};
+
+template <int G>
+__device__ __forceinline__ void load_rows16(Bits16<G>& f, const uint16_t* base, size_t ld, unsigned u0, unsigned v0, unsigned U, unsigned V, bool vec)
+{
+    const int lane = threadIdx.x & 31, q = lane & 3;
+    const unsigned u = u0 + lane / 4;
+    if (G == 4 && vec && v0 + 32 <= V) {
+        const uint16_t* p = base + (size_t)u * ld + v0 + 8 * q;
 #pragma unroll
-            for (int j = 0; j < CH; j++) y[j] = x[j];
-            if (epi.transposed()) epi.template combine<CH>(st, z, u, v0, s.V, y);
+        for (int g = 0; g < 4; g++, p += 8 * ld)
+            if (u + 8 * g < U) *reinterpret_cast<uint4*>(f.h[g]) = *reinterpret_cast<const uint4*>(p);
+    } else {
+        const uint16_t* p = base + (size_t)u * ld + v0 + 2 * q;
 #pragma unroll
-            for (int j = 0; j < CH; j++)
-                if (v0 + j < s.V) epi.column(st, z, u, v0 + j, y[j]);
-        }
-        if (epi.transposed()) return;
-    }
-    if (CH < 32) {                                        // narrow slices: each lane stores its own row
-        const unsigned u = u0 + lane;
-        if (u < s.U) {
+        for (int g = 0; g < 4; g++, p += 8 * ld) {
+            if (u + 8 * g >= U) continue;
 #pragma unroll
-            for (int j = 0; j < CH; j += 8) {
-                constexpr int W = CH < 8 ? CH : 8;
-                float y[8] = {};
-#pragma unroll
-                for (int i = 0; i < W; i++) y[i] = x[j + i];
-                if (v0 + j < s.V) epi.segment(st, z, u, v0 + j, min((unsigned)W, s.V - v0 - j), y);
+            for (int k = 0; k < G; k++) {
+                const unsigned v = v0 + 8 * k + 2 * q;
+                if (vec && v + 2 <= V) f.h[g][k] = *reinterpret_cast<const uint32_t*>(p + 8 * k);
+                else f.h[g][k] = (v < V ? p[8 * k] : 0u) | (v + 1 < V ? (uint32_t)p[8 * k + 1] << 16 : 0u);
             }
         }
-        return;
     }
-    // 32 x 32 through shared memory: 16-byte pieces, piece c of row r at c ^ (r & 7), so that both the row-wise writes and the
-    // reads (4 lanes per row, 8 values each) are free of bank conflicts.
-    float4* b4 = reinterpret_cast<float4*>(buf);
-    __syncwarp();
+}
+// What load_rows16 brought by rows, as fragments (all lanes of the warp).
+template <int G>
+__device__ __forceinline__ void rows_to_fragments(Bits16<G>& f, unsigned v0, unsigned V, bool vec)
+{
+    if constexpr (G == 4) {
+        if (vec && v0 + 32 <= V) {
 #pragma unroll
-    for (int c = 0; c < CH / 4; c++) b4[lane * 8 + (c ^ (lane & 7))] = make_float4(x[4 * c], x[4 * c + 1], x[4 * c + 2], x[4 * c + 3]);
-    __syncwarp();
-    const unsigned v = v0 + (lane & 3) * 8;
+            for (int g = 0; g < 4; g++) quad_transpose(f.h[g]);
+        }
+    }
+}
+template <int G>
+__device__ __forceinline__ void store_rows16(Bits16<G>& f, uint16_t* base, size_t ld, unsigned u0, unsigned v0, unsigned U, unsigned V, bool vec)
+{
+    const int lane = threadIdx.x & 31, q = lane & 3;
+    const unsigned u = u0 + lane / 4;
+    if constexpr (G == 4) {
+        if (vec && v0 + 32 <= V) {
+            uint16_t* p = base + (size_t)u * ld + v0 + 8 * q;
 #pragma unroll
-    for (int it = 0; it < 4; it++) {
-        const int r = it * 8 + lane / 4;
-        const unsigned u = u0 + r;
-        const float4 a = b4[r * 8 + ((2 * (lane & 3)) ^ (r & 7))], b = b4[r * 8 + ((2 * (lane & 3) + 1) ^ (r & 7))];
-        float y[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-        if (u < s.U && v < s.V) epi.segment(st, z, u, v, min(8u, s.V - v), y);
+            for (int g = 0; g < 4; g++, p += 8 * ld) {
+                quad_transpose(f.h[g]);
+                if (u + 8 * g < U) *reinterpret_cast<uint4*>(p) = make_uint4(f.h[g][0], f.h[g][1], f.h[g][2], f.h[g][3]);
+            }
+            return;
+        }
+    }
+    uint16_t* p = base + (size_t)u * ld + v0 + 2 * q;
+#pragma unroll
+    for (int g = 0; g < 4; g++, p += 8 * ld) {
+        if (u + 8 * g >= U) continue;
+#pragma unroll
+        for (int k = 0; k < G; k++) {
+            const unsigned v = v0 + 8 * k + 2 * q;
+            if (vec && v + 2 <= V) *reinterpret_cast<uint32_t*>(p + 8 * k) = f.h[g][k];
+            else {
+                if (v < V) p[8 * k] = (uint16_t)f.h[g][k];
+                if (v + 1 < V) p[8 * k + 1] = (uint16_t)(f.h[g][k] >> 16);
+            }
+        }
+    }
+}
+// The chunk transposed: 8 G lines of 32 values.  Blocks are transposed here; the lines v run over k, and the 32 rows u along a line.
+template <int G>
+__device__ __forceinline__ void store_columns16(const Bits16<G>& f, uint16_t* base, size_t ld, unsigned u0, unsigned v0, unsigned U, unsigned V, bool vec)
+{
+    const int lane = threadIdx.x & 31, q = lane & 3;
+    const unsigned v = v0 + lane / 4;
+#pragma unroll
+    for (int k = 0; k < G; k++) {
+        uint32_t r[4];
+#pragma unroll
+        for (int g = 0; g < 4; g++) r[g] = block_transpose(f.h[g][k]);
+        uint16_t* p = base + (size_t)(v + 8 * k) * ld + u0;
+        if (vec && u0 + 32 <= U) {
+            quad_transpose(r);
+            if (v + 8 * k < V) *reinterpret_cast<uint4*>(p + 8 * q) = make_uint4(r[0], r[1], r[2], r[3]);
+        } else if (v + 8 * k < V) {
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                const unsigned u = u0 + 8 * g + 2 * q;
+                if (u < U) p[8 * g + 2 * q] = (uint16_t)r[g];
+                if (u + 1 < U) p[8 * g + 2 * q + 1] = (uint16_t)(r[g] >> 16);
+            }
+        }
     }
 }
 
@@ -290,15 +363,35 @@ __device__ __forceinline__ void mma_slab(uint32_t sp, uint32_t tmem_d, bool firs
         umma<KIND, CG>(tmem_d, pd + ks * (32 >> 4), qd + ks * (QMN ? (16 * 128) >> 4 : 32 >> 4), idesc, !(first && ks == 0));
 }
 
+// 32 x 32 accumulators at a tensor-memory address (lane, column), as numbers.
+template <int KIND>
+__device__ __forceinline__ void read_chunk(float (&x)[4][4][2], uint32_t taddr)
+{
+    uint32_t a[16], b[16];
+    __syncwarp();
+    tmem_ld_16x32(taddr, a);
+    tmem_ld_16x32(taddr + (16u << 16), b);
+    tmem_ld_wait();
+#pragma unroll
+    for (int k = 0; k < 4; k++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            x[0][k][e] = acc_value<KIND>(a[4 * k + e]);
+            x[1][k][e] = acc_value<KIND>(a[4 * k + 2 + e]);
+            x[2][k][e] = acc_value<KIND>(b[4 * k + e]);
+            x[3][k][e] = acc_value<KIND>(b[4 * k + 2 + e]);
+        }
+}
+
 template <int BN, int CG>
 constexpr int stage_bytes() { return (BM + BN / CG) * SLAB_BYTES; }
 template <int BN, int CG>
 constexpr int persistent_stages()
 {
-    return (232448 - 1024 - 512 - EPI_WARPS * STAGE_BUF) / stage_bytes<BN, CG>();
+    return (232448 - 1024 - 512) / stage_bytes<BN, CG>();
 }
 template <int BN, int CG>
-constexpr int persistent_smem() { return persistent_stages<BN, CG>() * stage_bytes<BN, CG>() + EPI_WARPS * STAGE_BUF + 1024 + 512; }
+constexpr int persistent_smem() { return persistent_stages<BN, CG>() * stage_bytes<BN, CG>() + 1024 + 512; }
 
 // ---------------------------------------------------------------------------------------------------------------------
 // Persistent kernel
@@ -312,8 +405,7 @@ narrow_persistent_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_
     constexpr uint32_t TMEM_COLS = 2 * BN < 32 ? 32 : 2 * BN;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    float* bufs = reinterpret_cast<float*>(smem + STAGES * STAGE);
-    uint64_t* full = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE + EPI_WARPS * STAGE_BUF);
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE);
     uint64_t* empty = full + STAGES;
     uint64_t* acc_full = empty + STAGES;
     uint64_t* acc_empty = acc_full + 2;
@@ -344,6 +436,7 @@ narrow_persistent_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_
     if (CG == 2) cluster_sync();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
+    pdl_launch_dependents();
     pdl_wait();
 
     if (warp == 0) {
@@ -385,25 +478,26 @@ narrow_persistent_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_
             }
         }
     } else {
-        const int ew = warp - 2, quarter = warp & 3, half = ew / 4;
-        float* buf = bufs + ew * (STAGE_BUF / 4);
+        const int quarter = warp & 3, half = (warp - 2) / 4;
         unsigned n = 0;
         for (unsigned t = group; t < total; t += groups, n++) {
             unsigned tu, tv;
             const unsigned z = t / s.tiles;
             tile_coords(s, t - z * s.tiles, tu, tv);
             const unsigned a = n & 1;
+            const unsigned u0 = tu * BM * CG + rank * BM + quarter * 32;
+            constexpr int CHUNKS = BN / 32 / 2;               // per half
+            const unsigned v0 = tv * BN + half * CHUNKS * 32;
+            typename Epi::State st;
+            epi.begin(st, s, z, u0);
+            typename Epi::template Pre<4> pre;
+            epi.fetch(pre, s, z, u0, v0);
             if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[a], (n >> 1) & 1))) break;
             tc_fence_after();
-            const unsigned u0 = tu * BM * CG + rank * BM + quarter * 32;
-            typename Epi::State st;
-            const float factor = epi.begin(st, z, u0 + lane < s.U ? u0 + lane : s.U - 1);
-            constexpr int CHUNKS = BN / 32 / 2;               // per half
 #pragma unroll 1
             for (int c = 0; c < CHUNKS; c++) {
-                const int col = (half * CHUNKS + c) * 32;
-                uint32_t r[32];
-                tmem_ld32(tmem + ((uint32_t)(32 * quarter) << 16) + a * BN + col, r);
+                float x[4][4][2];
+                read_chunk<KIND>(x, tmem + ((uint32_t)(32 * quarter) << 16) + a * BN + (half * CHUNKS + c) * 32);
                 if (c == CHUNKS - 1) {                        // accumulator read: hand it back
                     tc_fence_before();
                     __syncwarp();
@@ -412,10 +506,7 @@ narrow_persistent_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_
                         else mbar_arrive(&acc_empty[a]);
                     }
                 }
-                float x[32];
-#pragma unroll
-                for (int j = 0; j < 32; j++) x[j] = factor * acc_value<KIND>(r[j]);
-                epilogue_chunk<Epi, 32>(epi, st, s, buf, z, u0, tv * BN + col, s.tri && tu != tv, x);
+                epi.chunk(st, pre, s, z, u0, v0 + c * 32, c + 1 < CHUNKS ? v0 + (c + 1) * 32 : ~0u, s.tri && tu != tv, x);
             }
             epi.end(st, z, t);
         }
@@ -444,13 +535,14 @@ narrow_split_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_const
 {
     constexpr int STAGES = split_stages<BN>(), STAGE = stage_bytes<BN, 1>();
     constexpr uint32_t TMEM_COLS = BN;
-    constexpr int SL = BN / S;                                    // columns each rank sums and finishes
+    // Column groups of 8 that a rank sums and finishes; with S > BN / 8 the last ranks have none.
+    constexpr int GROUPS = BN / 8, OWNERS = S < GROUPS ? S : GROUPS, OWN = GROUPS / OWNERS;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    // The ring is free once the products of every CTA of the cluster are done: the partial sums and the store buffers use it again.
-    uint32_t* part = reinterpret_cast<uint32_t*>(smem);                                // [S][SL][BM], written by all ranks
-    float* bufs = reinterpret_cast<float*>(smem + BN * BM * 4);
-    static_assert(BN * BM * 4 + EPI_WARPS * STAGE_BUF <= STAGES * STAGE, "the ring holds the partial sums and the store buffers");
+    // The ring is free once the products of every CTA of the cluster are done: the partial sums use it again, as fragments:
+    // [S ranks][4 quarters][OWN groups][4 g][32 lanes] pairs.
+    uint2* part = reinterpret_cast<uint2*>(smem);
+    static_assert(S * OWN * 8 * BM * 4 <= STAGES * STAGE, "the ring holds the partial sums");
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE);
     uint64_t* empty = full + STAGES;
     uint64_t* acc_full = empty + STAGES;
@@ -479,6 +571,7 @@ narrow_split_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_const
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
+    pdl_launch_dependents();
     pdl_wait();
 
     if (warp == 0) {
@@ -502,38 +595,42 @@ narrow_split_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_const
             umma_commit<1>(acc_full);
         }
     }
-    const int ew = warp - 2, quarter = warp & 3, half = ew / 4;
+    const int quarter = warp & 3, half = (warp - 2) / 4;
     const unsigned u0 = tu * BM + quarter * 32;
     const bool mirror = s.tri && tu != tv;
     typename Epi::State st;
-    float factor = 0.f;
     bool ok = true;
     if (warp >= 2) {
-        factor = epi.begin(st, z, u0 + lane < s.U ? u0 + lane : s.U - 1);
+        epi.begin(st, s, z, u0);
         ok = __all_sync(0xffffffffu, mbar_wait(acc_full, 0));
         tc_fence_after();
     }
     __syncwarp();
     if (S > 1) cluster_sync();                                    // the products of all CTAs of the cluster are done
-    if (warp >= 2) {
-        if (ok) {
-            constexpr int CHUNKS = BN / 32;
+    if (warp >= 2 && ok) {
 #pragma unroll 1
-            for (int c = half; c < CHUNKS; c += 2) {
-                uint32_t r[32];
-                tmem_ld32(tmem + ((uint32_t)(32 * quarter) << 16) + c * 32, r);
-                if (S == 1) {
-                    float x[32];
+        for (int c = half; c < BN / 32; c += 2) {
+            typename Epi::template Pre<4> pre;
+            if (S == 1) epi.fetch(pre, s, z, u0, tv * BN + c * 32);
+            const uint32_t taddr = tmem + ((uint32_t)(32 * quarter) << 16) + c * 32;
+            if (S == 1) {
+                float x[4][4][2];
+                read_chunk<KIND>(x, taddr);
+                epi.chunk(st, pre, s, z, u0, tv * BN + c * 32, ~0u, mirror, x);
+            } else {
+                uint32_t a[16], b[16];
+                __syncwarp();
+                tmem_ld_16x32(taddr, a);
+                tmem_ld_16x32(taddr + (16u << 16), b);
+                tmem_ld_wait();
 #pragma unroll
-                    for (int j = 0; j < 32; j++) x[j] = factor * acc_value<KIND>(r[j]);
-                    epilogue_chunk<Epi, 32>(epi, st, s, bufs + ew * (STAGE_BUF / 4), z, u0, tv * BN + c * 32, mirror, x);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 32; j++) {
-                        const int col = c * 32 + j, owner = col / SL;
-                        const uint32_t local = smem_u32(part + ((rank * SL + col % SL) * BM + quarter * 32 + lane));
-                        st_cluster(map_shared(local, (uint32_t)owner), r[j]);
-                    }
+                for (int k = 0; k < 4; k++) {
+                    const int group = c * 4 + k;
+                    const uint32_t to = map_shared(smem_u32(part + (((rank * 4 + quarter) * OWN + group % OWN) * 4) * 32 + lane), group / OWN);
+                    st_cluster(to, a[4 * k], a[4 * k + 1]);
+                    st_cluster(to + 256, a[4 * k + 2], a[4 * k + 3]);
+                    st_cluster(to + 512, b[4 * k], b[4 * k + 1]);
+                    st_cluster(to + 768, b[4 * k + 2], b[4 * k + 3]);
                 }
             }
         }
@@ -541,28 +638,32 @@ narrow_split_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_const
     if (S > 1) {
         __syncwarp();
         cluster_sync();
-        if (warp >= 2 && ok) {
-            // columns of this rank's slice, CH at a time; the two warps of a quarter take turns
-            constexpr int CH = SL < 32 ? SL : 32;
+        if (warp >= 2 && ok && rank < OWNERS) {
+            constexpr int G = OWN < 4 ? OWN : 4;                  // groups per chunk; the two warps of a quarter take turns
 #pragma unroll 1
-            for (int c = half; c < SL / CH; c += 2) {
-                float x[CH];
+            for (int c = half; c < OWN / G; c += 2) {
+                const unsigned v0 = tv * BN + rank * (OWN * 8) + c * (G * 8);
+                typename Epi::template Pre<G> pre;
+                epi.fetch(pre, s, z, u0, v0);
+                float x[4][G][2];
 #pragma unroll
-                for (int j = 0; j < CH; j++) {
-                    const uint32_t* p = part + (c * CH + j) * BM + quarter * 32 + lane;
-                    if (KIND == KIND_I8) {
-                        int a = 0;
+                for (int k = 0; k < G; k++)
 #pragma unroll
-                        for (int q = 0; q < S; q++) a += (int)p[q * SL * BM];
-                        x[j] = factor * (float)a;
-                    } else {
-                        float a = 0.f;
+                    for (int g = 0; g < 4; g++) {
+                        const uint2* p = part + ((quarter * OWN + c * G + k) * 4 + g) * 32 + lane;
+                        if (KIND == KIND_I8) {
+                            int i0 = 0, i1 = 0;
 #pragma unroll
-                        for (int q = 0; q < S; q++) a += __uint_as_float(p[q * SL * BM]);
-                        x[j] = factor * a;
+                            for (int q = 0; q < S; q++) { const uint2 w = p[q * 4 * OWN * 4 * 32]; i0 += (int)w.x; i1 += (int)w.y; }
+                            x[g][k][0] = (float)i0; x[g][k][1] = (float)i1;
+                        } else {
+                            float f0 = 0.f, f1 = 0.f;
+#pragma unroll
+                            for (int q = 0; q < S; q++) { const uint2 w = p[q * 4 * OWN * 4 * 32]; f0 += __uint_as_float(w.x); f1 += __uint_as_float(w.y); }
+                            x[g][k][0] = f0; x[g][k][1] = f1;
+                        }
                     }
-                }
-                epilogue_chunk<Epi, CH>(epi, st, s, bufs + ew * (STAGE_BUF / 4), z, u0, tv * BN + rank * SL + c * CH, mirror, x);
+                epi.chunk(st, pre, s, z, u0, v0, ~0u, mirror, x);
             }
         }
     }
@@ -615,12 +716,16 @@ cudaError_t launch(Kernel kernel, unsigned grid, unsigned cluster, int smem, cud
     cfg.blockDim = dim3(THREADS);
     cfg.dynamicSmemBytes = (size_t)smem;
     cfg.stream = st;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = cluster;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    // chained: the kernel before it on the stream is one of a chain of short products; it may start (barriers, tensor memory,
+    // descriptors) while that one drains, and waits for its results in pdl_wait().
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = Epi::kChained ? 2 : 1;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, mp, mq, s, epi);
     if (e == cudaSuccess) count_launch();
     return e;
@@ -659,25 +764,34 @@ cudaError_t run_split(const Operand& p, const Operand& q, Shape s, const Epi& ep
     return launch(kernel, s.tiles * s.batch * S, S, smem, st, mp, mq, s, epi);
 }
 
-// How a product of more than 64 columns runs.  Estimated clocks: rounds of tiles times (slabs x clocks per slab + what a tile costs besides).
-//   pairs:  256 x 256 tiles on pairs of CTAs, 512 clocks per slab
-//   single: 128 x 128 tiles, persistent, 300 clocks per slab (both operands are read from shared memory at its full rate)
-//   split:  128 x 128 tiles, k over S CTAs of a cluster
+// How a product of more than 64 columns runs.  Estimated clocks, fitted to measurements: rounds of tiles times slabs and epilogues.
+// Operands come from L2, which gives a slab of 128 x 128 tiles every 570 clocks (32 KB per SM) and one of 256 x 256 tiles every 650
+// (32 KB per SM for twice the products) when all SMs ask at once; a lone tile gets a slab in about 300.
+//   pairs:  256 x 256 tiles on pairs of CTAs
+//   single: 128 x 128 tiles, persistent
+//   split:  128 x 128 tiles, k (and the epilogue's columns) over S CTAs of a cluster
 struct Plan { bool pairs; unsigned split; };         // split == 0: persistent
 inline Plan choose_plan(unsigned U, unsigned V, unsigned K, unsigned batch, int tri, int kind)
 {
-    const double sms = sm_count(), nk = (K + slab_k(kind) - 1) / slab_k(kind);
+    const unsigned sms = (unsigned)sm_count(), nk = (K + slab_k(kind) - 1) / slab_k(kind);
     auto tiles = [&](unsigned b) {
-        const double tu = (U + b - 1) / b, tv = (V + b - 1) / b;
-        return batch * (tri ? tu * (tu + 1) / 2 : tu * tv);
+        const unsigned long long tu = (U + b - 1) / b, tv = (V + b - 1) / b;
+        return (double)(batch * (tri ? tu * (tu + 1) / 2 : tu * tv));
     };
-    auto rounds = [](double work, double slots) { const double r = work / slots; return (double)(unsigned long long)r + (r > (double)(unsigned long long)r); };
+    const double t128 = tiles(128), t256 = tiles(256);
+    auto slab = [&](double busy, double all) { const double f = busy / sms; return 300 + (all - 300) * (f < 1 ? f : 1); };
+    auto loop = [](double per_tile, double epilogue, double rounds) {     // persistent: the epilogue runs under the next tile's slabs
+        const double longer = per_tile > epilogue ? per_tile : epilogue;
+        return per_tile + (rounds - 1) * longer + epilogue;
+    };
+    const double epi = tri ? 1500 : 1200;                                 // per chunk of 32 columns and warp
     Plan best{true, 0};
-    double least = rounds(tiles(256), (double)((int)sms / 2)) * (nk * 512 + 500) + 4000;
-    const double t128 = tiles(128), single = rounds(t128, sms) * (nk * 300 + 500) + 3000;
+    double least = loop(nk * slab(2 * t256, 650), 4 * epi, std::ceil(t256 / (sms / 2))) + 2000;
+    const double single = loop(nk * slab(t128, 570), 2 * epi, std::ceil(t128 / sms)) + 1500;
     if (single < least) { least = single; best = {false, 0}; }
     for (unsigned s = 1; s <= 8 && s <= nk; s *= 2) {
-        const double c = rounds(t128 * s, sms) * ((double)(((unsigned)nk + s - 1) / s) * 300 + 3000 + (s > 1 ? 1500 : 0));
+        const double chunks = s <= 2 ? 2.0 / s : 1;
+        const double c = std::ceil(t128 * s / sms) * (((nk + s - 1) / s) * slab(t128 * s, 570) + chunks * epi + 1500 + (s > 1 ? 1500 : 0));
         if (c < least) { least = c; best = {false, s}; }
     }
     return best;

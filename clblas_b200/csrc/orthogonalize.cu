@@ -40,20 +40,8 @@ template <> __device__ __forceinline__ float to_f(float v) { return v; }
 template <> __device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
 template <> __device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
 
-struct alignas(16) Half8 { __half2 h[4]; };
-__device__ __forceinline__ void load8(const __half* p, float (&x)[8])
-{
-    const Half8 v = *reinterpret_cast<const Half8*>(p);
-#pragma unroll
-    for (int i = 0; i < 4; i++) { const float2 f = __half22float2(v.h[i]); x[2 * i] = f.x; x[2 * i + 1] = f.y; }
-}
-__device__ __forceinline__ void store8(__half* p, const float (&x)[8])
-{
-    Half8 v;
-#pragma unroll
-    for (int i = 0; i < 4; i++) v.h[i] = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
-    *reinterpret_cast<Half8*>(p) = v;
-}
+__device__ __forceinline__ uint32_t pack(float a, float b) { const __half2 h = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t*>(&h); }
+__device__ __forceinline__ float2 unpack(uint32_t h) { return __half22float2(*reinterpret_cast<const __half2*>(&h)); }
 
 // ---- norm and split ---------------------------------------------------------------------------------------------------
 
@@ -138,114 +126,158 @@ __global__ void __launch_bounds__(256) split_kernel(const T* __restrict__ G, siz
 }
 
 // ---- epilogues ----------------------------------------------------------------------------------------------------------
-// Segments are eight aligned columns here (slices of at least 8 columns, workspaces with a pitch of a multiple of 8): pieces of the
-// workspaces are read and written whole, what lies beyond V is padding that no product reads.
 
 // The shift t: the mean diagonal of X X', once most singular values have come near one; 0 before (and for a matrix of NaN, whose
 // sum says nothing).  While X is dominated by a few directions the shift would put roundings of t on all the others
 // (rank 8 of 100: 3e-3 with t from the first step on, 7e-4 from t = 0.2 on).
 __device__ __forceinline__ float shift_of(const u64* sums, size_t at, float inv_n)
 {
-    const float t = (float)((double)sums[at] * (1.0 / SUM_UNIT)) * inv_n;
+    const float t = (float)((double)__ldcg(sums + at) * (1.0 / SUM_UNIT)) * inv_n;       // past L1: a neighbour is added to meanwhile
     return t >= 0.2f ? t : 0.f;
 }
 
+// The workspaces have a pitch of a multiple of 8 elements: every row piece is aligned.
+__device__ __forceinline__ uint16_t* bits(__half* p) { return reinterpret_cast<uint16_t*>(p); }
+__device__ __forceinline__ const uint16_t* bits(const __half* p) { return reinterpret_cast<const uint16_t*>(p); }
+
 struct EpiGram {                                           // A <- X X' - t I
-    static constexpr bool kMirror = true;
+    static constexpr bool kChained = true;
     struct State { float t; };
+    template <int G> struct Pre {};
     __half* A; size_t ld, stride;
     const u64* sums; int pitch;
     float inv_n;
-    __device__ bool transposed() const { return false; }
-    __device__ float begin(State& st, unsigned z, unsigned) const
+    __device__ void begin(State& st, const Shape&, unsigned z, unsigned) const { st.t = SA * shift_of(sums, (size_t)z * pitch, inv_n); }
+    template <int G> __device__ void fetch(Pre<G>&, const Shape&, unsigned, unsigned, unsigned) const {}
+    template <int G>
+    __device__ void chunk(State& st, Pre<G>&, const Shape& s, unsigned z, unsigned u0, unsigned v0, unsigned, bool mirror, float (&x)[4][G][2]) const
     {
-        st.t = SA * shift_of(sums, (size_t)z * pitch, inv_n);
-        return SA / (SX * SX);
-    }
-    template <int CH> __device__ void combine(State&, unsigned, unsigned, unsigned, unsigned, float (&)[CH]) const {}
-    __device__ void column(State&, unsigned z, unsigned u, unsigned v, float x) const { A[z * stride + (size_t)v * ld + u] = __float2half_rn(x); }
-    __device__ void segment(State& st, unsigned z, unsigned u, unsigned v, unsigned n, float (&x)[8]) const
-    {
+        const int lane = threadIdx.x & 31;
+        const int off = (int)(u0 + lane / 4) - (int)(v0 + 2 * (lane & 3));      // row - column of x[0][0][0]
+        Bits16<G> o;
 #pragma unroll
-        for (int i = 0; i < 8; i++) if (u == v + i) x[i] -= st.t;
-        store8(A + z * stride + (size_t)u * ld + v, x);
+        for (int g = 0; g < 4; g++)
+#pragma unroll
+            for (int k = 0; k < G; k++) {
+                float a = x[g][k][0] * (SA / (SX * SX)), b = x[g][k][1] * (SA / (SX * SX));
+                const int d = off + 8 * (g - k);
+                if (d == 0) a -= st.t;
+                if (d == 1) b -= st.t;
+                o.h[g][k] = pack(a, b);
+            }
+        if (mirror) store_columns16<G>(o, bits(A + z * stride), ld, u0, v0, s.U, s.V, true);
+        store_rows16<G>(o, bits(A + z * stride), ld, u0, v0, s.U, s.V, true);
     }
     __device__ void end(State&, unsigned, unsigned) const {}
 };
 
 struct EpiSquare {                                         // P <- (b + 2 c t) A + c A^2
-    static constexpr bool kMirror = true;
+    static constexpr bool kChained = true;
     struct State { float b; };
+    template <int G> struct Pre { Bits16<G> a; };
     const __half* A; __half* P; size_t ld, stride;
     const u64* sums; int pitch;
     float inv_n, b, c;
-    __device__ bool transposed() const { return false; }
-    __device__ float begin(State& st, unsigned z, unsigned) const
+    __device__ void begin(State& st, const Shape&, unsigned z, unsigned) const { st.b = b + 2.f * c * shift_of(sums, (size_t)z * pitch, inv_n); }
+    template <int G>
+    __device__ void fetch(Pre<G>& p, const Shape& s, unsigned z, unsigned u0, unsigned v0) const
     {
-        st.b = b + 2.f * c * shift_of(sums, (size_t)z * pitch, inv_n);
-        return c / SA;
+        load_rows16<G>(p.a, bits(A + z * stride), ld, u0, v0, s.U, s.V, true);
     }
-    template <int CH> __device__ void combine(State&, unsigned, unsigned, unsigned, unsigned, float (&)[CH]) const {}
-    __device__ void column(State& st, unsigned z, unsigned u, unsigned v, float x) const
+    template <int G>
+    __device__ void chunk(State& st, Pre<G>& p, const Shape& s, unsigned z, unsigned u0, unsigned v0, unsigned v_next, bool mirror, float (&x)[4][G][2]) const
     {
-        const size_t at = z * stride + (size_t)v * ld + u;
-        P[at] = __float2half_rn(fmaf(st.b, __half2float(A[at]), x));
-    }
-    __device__ void segment(State& st, unsigned z, unsigned u, unsigned v, unsigned n, float (&x)[8]) const
-    {
-        const size_t at = z * stride + (size_t)u * ld + v;
-        float a[8];
-        load8(A + at, a);
+        rows_to_fragments<G>(p.a, v0, s.V, true);
+        const float f = c / SA;
+        Bits16<G> o;
 #pragma unroll
-        for (int i = 0; i < 8; i++) a[i] = fmaf(st.b, a[i], x[i]);
-        store8(P + at, a);
+        for (int g = 0; g < 4; g++)
+#pragma unroll
+            for (int k = 0; k < G; k++) {
+                const float2 a = unpack(p.a.h[g][k]);
+                o.h[g][k] = pack(fmaf(st.b, a.x, f * x[g][k][0]), fmaf(st.b, a.y, f * x[g][k][1]));
+            }
+        if (v_next != ~0u) fetch<G>(p, s, z, u0, v_next);
+        if (mirror) store_columns16<G>(o, bits(P + z * stride), ld, u0, v0, s.U, s.V, true);
+        store_rows16<G>(o, bits(P + z * stride), ld, u0, v0, s.U, s.V, true);
     }
     __device__ void end(State&, unsigned, unsigned) const {}
 };
 
 // Common part of the two updates: y = (a + b t + c t^2) X + P X, times SX.  P is P, or A with factor b when c == 0.
 struct UpdateTerm {
-    const __half* hi; const __half* lo; size_t ldx, stride_x;
+    const __half* hi; const __half* lo; size_t ld, stride;
     const u64* sums; int pitch;
     float inv_n, a, b, c;
+    template <int G> struct Pre { Bits16<G> h, l; };
+    template <int G>
+    __device__ void fetch(Pre<G>& p, const Shape& s, unsigned z, unsigned u0, unsigned v0) const
+    {
+        load_rows16<G>(p.h, bits(hi + z * stride), ld, u0, v0, s.U, s.V, true);
+        load_rows16<G>(p.l, bits(lo + z * stride), ld, u0, v0, s.U, s.V, true);
+    }
     __device__ float coefficient(unsigned z) const
     {
         const float t = shift_of(sums, (size_t)z * pitch, inv_n);
         return a + t * (b + c * t);
     }
-    __device__ float factor() const { return (c == 0.f ? b : 1.f) / SA; }
+    // x <- scale * (coefficient X + P X)
+    template <int G>
+    __device__ void add(Pre<G>& p, const Shape& s, unsigned v0, float coefficient, float scale, float (&x)[4][G][2]) const
+    {
+        rows_to_fragments<G>(p.h, v0, s.V, true);
+        rows_to_fragments<G>(p.l, v0, s.V, true);
+        const float f = scale * ((c == 0.f ? b : 1.f) / SA), w = scale * coefficient;
+#pragma unroll
+        for (int g = 0; g < 4; g++)
+#pragma unroll
+            for (int k = 0; k < G; k++) {
+                const float2 h = unpack(p.h.h[g][k]), l = unpack(p.l.h[g][k]);
+                x[g][k][0] = fmaf(w, h.x + l.x, f * x[g][k][0]);
+                x[g][k][1] = fmaf(w, h.y + l.y, f * x[g][k][1]);
+            }
+    }
 };
 
 struct EpiUpdate {
-    static constexpr bool kMirror = false;
+    static constexpr bool kChained = true;
     struct State { float a, sum; };
+    template <int G> using Pre = UpdateTerm::Pre<G>;
     UpdateTerm t;
-    __half* hi; __half* lo;                                // lo may be the one that is read: each place is read and written by one thread
+    __half* hi; __half* lo;                                // lo may be the one that is read: each place is read, then written, by one thread
     u64* next;                                             // sums of the new X
-    __device__ bool transposed() const { return false; }
-    __device__ float begin(State& st, unsigned z, unsigned) const
+    __device__ void begin(State& st, const Shape&, unsigned z, unsigned) const
     {
         st.a = t.coefficient(z);
         st.sum = 0.f;
-        return t.factor();
     }
-    template <int CH> __device__ void combine(State&, unsigned, unsigned, unsigned, unsigned, float (&)[CH]) const {}
-    __device__ void column(State&, unsigned, unsigned, unsigned, float) const {}
-    __device__ void segment(State& st, unsigned z, unsigned u, unsigned v, unsigned n, float (&x)[8]) const
+    template <int G> __device__ void fetch(Pre<G>& p, const Shape& s, unsigned z, unsigned u0, unsigned v0) const { t.fetch<G>(p, s, z, u0, v0); }
+    template <int G>
+    __device__ void chunk(State& st, Pre<G>& p, const Shape& s, unsigned z, unsigned u0, unsigned v0, unsigned v_next, bool, float (&x)[4][G][2]) const
     {
-        const size_t at = z * t.stride_x + (size_t)u * t.ldx + v;
-        float h[8], l[8];
-        load8(t.hi + at, h);
-        load8(t.lo + at, l);
+        t.add<G>(p, s, v0, st.a, 1.f, x);
+        if (v_next != ~0u) fetch<G>(p, s, z, u0, v_next);
+        const int lane = threadIdx.x & 31;
+        Bits16<G> h, l;
+        float sum = 0.f;
+        const bool whole = u0 + 32 <= s.U && v0 + 8 * G <= s.V;
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            x[i] = fmaf(st.a, h[i] + l[i], x[i]);
-            h[i] = __half2float(__float2half_rn(x[i]));
-            l[i] = x[i] - h[i];
-            if (i < (int)n) st.sum = fmaf(x[i], x[i], st.sum);
-        }
-        store8(hi + at, h);
-        store8(lo + at, l);
+        for (int g = 0; g < 4; g++)
+#pragma unroll
+            for (int k = 0; k < G; k++) {
+                const float a = x[g][k][0], b = x[g][k][1];
+                h.h[g][k] = pack(a, b);
+                const float2 r = unpack(h.h[g][k]);
+                l.h[g][k] = pack(a - r.x, b - r.y);
+                // outside the matrix the accumulators are zero but the fetched values may be anything: chosen, not multiplied by zero
+                const unsigned v = v0 + 8 * k + 2 * (lane & 3);
+                const bool in = whole || u0 + 8 * g + lane / 4 < s.U;
+                sum += in && (whole || v < s.V) ? a * a : 0.f;
+                sum += in && (whole || v + 1 < s.V) ? b * b : 0.f;
+            }
+        st.sum += sum;
+        store_rows16<G>(h, bits(hi + z * t.stride), t.ld, u0, v0, s.U, s.V, true);
+        store_rows16<G>(l, bits(lo + z * t.stride), t.ld, u0, v0, s.U, s.V, true);
     }
     __device__ void end(State& st, unsigned z, unsigned) const
     {
@@ -259,71 +291,59 @@ struct EpiUpdate {
 };
 
 struct EpiOut {                                            // O <- alpha X + beta O
-    static constexpr bool kMirror = false;
+    static constexpr bool kChained = true;
     struct State { float a; };
+    template <int G> struct Pre { UpdateTerm::Pre<G> x; Bits16<G> o; };
     UpdateTerm t;
-    __nv_bfloat16* O; size_t ldo, stride_o;
+    uint16_t* O; size_t ldo, stride_o;                     // BF16
     float alpha, beta;
-    bool flip, vec;                                        // flip: element (u, v) at O[v * ldo + u]
-    __device__ bool transposed() const { return flip; }
-    __device__ float begin(State& st, unsigned z, unsigned) const
+    bool flip, vec;                                        // flip: element (u, v) at O[v * ldo + u]; vec: 16-byte accesses of O allowed
+    __device__ void begin(State& st, const Shape&, unsigned z, unsigned) const { st.a = t.coefficient(z); }
+    template <int G>
+    __device__ void fetch(Pre<G>& p, const Shape& s, unsigned z, unsigned u0, unsigned v0) const
     {
-        st.a = t.coefficient(z) * (alpha / SX);
-        return t.factor() * (alpha / SX);
+        t.fetch<G>(p.x, s, z, u0, v0);
+        if (beta != 0.f && !flip) load_rows16<G>(p.o, O + z * stride_o, ldo, u0, v0, s.U, s.V, vec);
     }
-    template <int CH>
-    __device__ void combine(State& st, unsigned z, unsigned u, unsigned v0, unsigned V, float (&x)[CH]) const
+    template <int G>
+    __device__ void chunk(State& st, Pre<G>& p, const Shape& s, unsigned z, unsigned u0, unsigned v0, unsigned v_next, bool, float (&x)[4][G][2]) const
     {
-        const size_t at = z * t.stride_x + (size_t)u * t.ldx + v0;
+        t.add<G>(p.x, s, v0, st.a, alpha / SX, x);
+        uint16_t* o = O + z * stride_o;
+        if (beta != 0.f) {
+            const int lane = threadIdx.x & 31;
+            if (flip) {                                    // fragments of the transposed matrix
 #pragma unroll
-        for (int j = 0; j < CH; j += 8) {
-            if (v0 + j >= V) break;
-            float h[8], l[8];
-            load8(t.hi + at + j, h);
-            load8(t.lo + at + j, l);
+                for (int g = 0; g < 4; g++)
 #pragma unroll
-            for (int i = 0; i < 8; i++) x[j + i] = fmaf(st.a, h[i] + l[i], x[j + i]);
-        }
-    }
-    __device__ void column(State&, unsigned z, unsigned u, unsigned v, float x) const
-    {
-        __nv_bfloat16* o = O + z * stride_o + (size_t)v * ldo + u;
-        if (beta != 0.f) x = fmaf(beta, __bfloat162float(*o), x);
-        *o = __float2bfloat16_rn(x);
-    }
-    __device__ void segment(State& st, unsigned z, unsigned u, unsigned v, unsigned n, float (&x)[8]) const
-    {
-        const size_t at = z * t.stride_x + (size_t)u * t.ldx + v;
-        __nv_bfloat16* o = O + z * stride_o + (size_t)u * ldo + v;
-        float h[8], l[8];
-        load8(t.hi + at, h);
-        load8(t.lo + at, l);
-#pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = fmaf(st.a, h[i] + l[i], x[i]);
-        if (vec && n == 8) {
-            uint4 raw;
-            __nv_bfloat162* p = reinterpret_cast<__nv_bfloat162*>(&raw);
-            if (beta != 0.f) {
-                raw = *reinterpret_cast<const uint4*>(o);
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float2 f = __bfloat1622float2(p[i]);
-                    x[2 * i] = fmaf(beta, f.x, x[2 * i]);
-                    x[2 * i + 1] = fmaf(beta, f.y, x[2 * i + 1]);
-                }
+                    for (int k = 0; k < G; k++) {
+                        const unsigned u = u0 + 8 * g + lane / 4, v = v0 + 8 * k + 2 * (lane & 3);
+                        const uint32_t a = u < s.U && v < s.V ? o[(size_t)v * ldo + u] : 0u, b = u < s.U && v + 1 < s.V ? o[(size_t)(v + 1) * ldo + u] : 0u;
+                        p.o.h[g][k] = a | b << 16;
+                    }
+            } else {
+                rows_to_fragments<G>(p.o, v0, s.V, vec);
             }
 #pragma unroll
-            for (int i = 0; i < 4; i++) p[i] = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
-            *reinterpret_cast<uint4*>(o) = raw;
-            return;
-        }
+            for (int g = 0; g < 4; g++)
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            if (i >= (int)n) break;
-            float y = x[i];
-            if (beta != 0.f) y = fmaf(beta, __bfloat162float(o[i]), y);
-            o[i] = __float2bfloat16_rn(y);
+                for (int k = 0; k < G; k++) {
+                    const float2 old = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&p.o.h[g][k]));
+                    x[g][k][0] = fmaf(beta, old.x, x[g][k][0]);
+                    x[g][k][1] = fmaf(beta, old.y, x[g][k][1]);
+                }
         }
+        if (v_next != ~0u) fetch<G>(p, s, z, u0, v_next);
+        Bits16<G> r;
+#pragma unroll
+        for (int g = 0; g < 4; g++)
+#pragma unroll
+            for (int k = 0; k < G; k++) {
+                const __nv_bfloat162 b = __floats2bfloat162_rn(x[g][k][0], x[g][k][1]);
+                r.h[g][k] = *reinterpret_cast<const uint32_t*>(&b);
+            }
+        if (flip) store_columns16<G>(r, o, ldo, u0, v0, s.U, s.V, vec);
+        else store_rows16<G>(r, o, ldo, u0, v0, s.U, s.V, vec);
     }
     __device__ void end(State&, unsigned, unsigned) const {}
 };
@@ -384,7 +404,7 @@ cudaError_t orthogonalize_typed(const OrthProblem& p, cudaStream_t s)
         if (k + 1 < p.steps) {
             e = run_planned<KIND_F16, true>(c != 0.f ? op : oa, ox, up_, EpiUpdate{t, hi[(k + 1) & 1], lo, sums + k + 1}, s);
         } else {
-            __nv_bfloat16* O = static_cast<__nv_bfloat16*>(p.O) + p.offO;
+            uint16_t* O = static_cast<uint16_t*>(p.O) + p.offO;
             const bool vec = aligned16(O) && p.ldo % 8 == 0 && (batch == 1 || p.strideO % 8 == 0);
             e = run_planned<KIND_F16, true>(c != 0.f ? op : oa, ox, up_, EpiOut{t, O, p.ldo, p.strideO, p.alpha, p.beta, flip, vec}, s);
         }
