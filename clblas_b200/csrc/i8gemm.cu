@@ -44,7 +44,7 @@ struct EpiScaled {
     T* C;
     size_t ld;
     bool trans;                     // element (u, v) at C[v * ld + u] instead of C[u * ld + v]
-    bool vec;                       // 16-byte accesses of C allowed
+    int align;                      // of C's lines: 16, 4 or 2 bytes (16-bit C); 8-byte accesses allowed when 8 or more (32-bit C)
 
     __device__ void begin(State& st, const Shape& s, unsigned, unsigned u0) const
     {
@@ -55,7 +55,9 @@ struct EpiScaled {
     template <int G>
     __device__ void fetch(Pre<G>& p, const Shape& s, unsigned, unsigned u0, unsigned v0) const
     {
-        if (sizeof(T) == 2 && beta != 0.f && !trans) load_rows16<G>(p.c, reinterpret_cast<const uint16_t*>(C), ld, u0, v0, s.U, s.V, vec);
+        if (sizeof(T) == 4 || beta == 0.f) return;
+        if (trans) load_columns16<G>(p.c, reinterpret_cast<const uint16_t*>(C), ld, u0, v0, s.U, s.V, align);
+        else load_rows16<G>(p.c, reinterpret_cast<const uint16_t*>(C), ld, u0, v0, s.U, s.V, align);
     }
     template <int G>
     __device__ void chunk(State& st, Pre<G>& p, const Shape& s, unsigned z, unsigned u0, unsigned v0, unsigned v_next, bool, float (&x)[4][G][2]) const
@@ -72,7 +74,7 @@ struct EpiScaled {
                 x[g][k][1] = x[g][k][1] * st.factor[g] * w1;
             }
         }
-        if (beta != 0.f && (trans || sizeof(T) == 4)) {             // C in fragments
+        if (sizeof(T) == 4 && beta != 0.f) {
             T old[4][G][2];
 #pragma unroll
             for (int g = 0; g < 4; g++)
@@ -89,8 +91,9 @@ struct EpiScaled {
                     for (int e = 0; e < 2; e++) x[g][k][e] = fmaf(beta, to_f(old[g][k][e]), x[g][k][e]);
         }
         if constexpr (sizeof(T) == 2) {
-            if (beta != 0.f && !trans) {
-                rows_to_fragments<G>(p.c, v0, s.V, vec);
+            if (beta != 0.f) {
+                if (trans) columns_to_fragments<G>(p.c);
+                else rows_to_fragments<G>(p.c, v0, s.V, align);
 #pragma unroll
                 for (int g = 0; g < 4; g++)
 #pragma unroll
@@ -106,8 +109,8 @@ struct EpiScaled {
             for (int g = 0; g < 4; g++)
 #pragma unroll
                 for (int k = 0; k < G; k++) o.h[g][k] = pack16<T>(x[g][k][0], x[g][k][1]);
-            if (trans) store_columns16<G>(o, reinterpret_cast<uint16_t*>(C), ld, u0, v0, s.U, s.V, vec);
-            else store_rows16<G>(o, reinterpret_cast<uint16_t*>(C), ld, u0, v0, s.U, s.V, vec);
+            if (trans) store_columns16<G>(o, reinterpret_cast<uint16_t*>(C), ld, u0, v0, s.U, s.V, align);
+            else store_rows16<G>(o, reinterpret_cast<uint16_t*>(C), ld, u0, v0, s.U, s.V, align);
         } else {                                                    // 32-bit: a quad's fragments fill 32 bytes of a row, eight lanes' 32 bytes of a column
 #pragma unroll
             for (int g = 0; g < 4; g++)
@@ -116,7 +119,7 @@ struct EpiScaled {
                     const unsigned v = v0 + 8 * k + 2 * q;
                     if (u + 8 * g >= s.U) continue;
                     float* c = reinterpret_cast<float*>(C) + at(u + 8 * g, v);
-                    if (!trans && vec && v + 2 <= s.V) *reinterpret_cast<float2*>(c) = make_float2(x[g][k][0], x[g][k][1]);
+                    if (!trans && align >= 8 && v + 2 <= s.V) *reinterpret_cast<float2*>(c) = make_float2(x[g][k][0], x[g][k][1]);
                     else {
                         if (v < s.V) *c = x[g][k][0];
                         if (v + 1 < s.V) c[trans ? ld : 1] = x[g][k][1];
@@ -228,7 +231,7 @@ cudaError_t multiply(const Operand& lines, const Operand& len, const float* s_li
 {
     // C is `lines.rows` lines of `len.rows` contiguous elements.
     const size_t L = lines.rows, W = len.rows, K = lines.inner;
-    const bool vec_c = aligned16(C) && (ldc * sizeof(T)) % 16 == 0;
+    const int align = sizeof(T) == 2 ? line_alignment(C, ldc, 0) : (reinterpret_cast<uintptr_t>(C) | (ldc * 4)) % 8 == 0 ? 8 : 4;
     const unsigned nk = (unsigned)((K + slab_k(KIND_I8) - 1) / slab_k(KIND_I8));
     const unsigned sms = (unsigned)sm_count();
     Shape s = {};
@@ -236,7 +239,7 @@ cudaError_t multiply(const Operand& lines, const Operand& len, const float* s_li
     s.batch = 1;
     auto normal = [&] {
         s.U = (unsigned)L; s.V = (unsigned)W;
-        return EpiScaled<T>{s_lines, s_len, alpha, beta, C, ldc, false, vec_c};
+        return EpiScaled<T>{s_lines, s_len, alpha, beta, C, ldc, false, align};
     };
     auto split_for = [&](unsigned bn, unsigned per_sm) {
         const size_t tiles = ((s.U + BM - 1) / BM) * (size_t)((s.V + bn - 1) / bn);
@@ -247,7 +250,7 @@ cudaError_t multiply(const Operand& lines, const Operand& len, const float* s_li
     if (L <= 128 && W > L) {
         // Few lines (decoding): the contiguous dimension supplies the 128 rows of the instruction, the lines its columns.
         s.U = (unsigned)W; s.V = (unsigned)L;
-        const EpiScaled<T> epi{s_len, s_lines, alpha, beta, C, ldc, true, vec_c};
+        const EpiScaled<T> epi{s_len, s_lines, alpha, beta, C, ldc, true, align};
         if (L <= 32) return run_split_by<KIND_I8, 32, false>(split_for(32, 2), len, lines, s, epi, st);
         if (L <= 64) return run_split_by<KIND_I8, 64, false>(split_for(64, 2), len, lines, s, epi, st);
         return run_split_by<KIND_I8, 128, false>(split_for(128, 1), len, lines, s, epi, st);

@@ -236,18 +236,19 @@ __device__ __forceinline__ uint32_t block_transpose(uint32_t v)
 }
 
 // 16-bit matrices (as raw bits): a lane's share of a chunk, by rows (16 bytes per 8 rows) or by fragments.
-// `vec`: base and pitch allow 16-byte accesses; without it, and for chunks narrower than 32 columns, fragments are accessed directly.
+// `align`: bytes by which base and pitch are aligned, 16, 4 or 2.  Below 16, at the matrix's edge and for chunks narrower than 32 columns
+// fragments are accessed directly, 4 or 2 bytes a lane.
 template <int G>
 struct Bits16 {
     uint32_t h[4][G];                                       // [g][k]: two values of row 8 g + lane / 4, columns 8 k + 2 (lane % 4)
 };
 
 template <int G>
-__device__ __forceinline__ void load_rows16(Bits16<G>& f, const uint16_t* base, size_t ld, unsigned u0, unsigned v0, unsigned U, unsigned V, bool vec)
+__device__ __forceinline__ void load_rows16(Bits16<G>& f, const uint16_t* base, size_t ld, unsigned u0, unsigned v0, unsigned U, unsigned V, int align)
 {
     const int lane = threadIdx.x & 31, q = lane & 3;
     const unsigned u = u0 + lane / 4;
-    if (G == 4 && vec && v0 + 32 <= V) {
+    if (G == 4 && align == 16 && v0 + 32 <= V) {
         const uint16_t* p = base + (size_t)u * ld + v0 + 8 * q;
 #pragma unroll
         for (int g = 0; g < 4; g++, p += 8 * ld)
@@ -260,7 +261,7 @@ __device__ __forceinline__ void load_rows16(Bits16<G>& f, const uint16_t* base, 
 #pragma unroll
             for (int k = 0; k < G; k++) {
                 const unsigned v = v0 + 8 * k + 2 * q;
-                if (vec && v + 2 <= V) f.h[g][k] = *reinterpret_cast<const uint32_t*>(p + 8 * k);
+                if (align >= 4 && v + 2 <= V) f.h[g][k] = *reinterpret_cast<const uint32_t*>(p + 8 * k);
                 else f.h[g][k] = (v < V ? p[8 * k] : 0u) | (v + 1 < V ? (uint32_t)p[8 * k + 1] << 16 : 0u);
             }
         }
@@ -268,22 +269,22 @@ __device__ __forceinline__ void load_rows16(Bits16<G>& f, const uint16_t* base, 
 }
 // What load_rows16 brought by rows, as fragments (all lanes of the warp).
 template <int G>
-__device__ __forceinline__ void rows_to_fragments(Bits16<G>& f, unsigned v0, unsigned V, bool vec)
+__device__ __forceinline__ void rows_to_fragments(Bits16<G>& f, unsigned v0, unsigned V, int align)
 {
     if constexpr (G == 4) {
-        if (vec && v0 + 32 <= V) {
+        if (align == 16 && v0 + 32 <= V) {
 #pragma unroll
             for (int g = 0; g < 4; g++) quad_transpose(f.h[g]);
         }
     }
 }
 template <int G>
-__device__ __forceinline__ void store_rows16(Bits16<G>& f, uint16_t* base, size_t ld, unsigned u0, unsigned v0, unsigned U, unsigned V, bool vec)
+__device__ __forceinline__ void store_rows16(Bits16<G>& f, uint16_t* base, size_t ld, unsigned u0, unsigned v0, unsigned U, unsigned V, int align)
 {
     const int lane = threadIdx.x & 31, q = lane & 3;
     const unsigned u = u0 + lane / 4;
     if constexpr (G == 4) {
-        if (vec && v0 + 32 <= V) {
+        if (align == 16 && v0 + 32 <= V) {
             uint16_t* p = base + (size_t)u * ld + v0 + 8 * q;
 #pragma unroll
             for (int g = 0; g < 4; g++, p += 8 * ld) {
@@ -300,7 +301,7 @@ __device__ __forceinline__ void store_rows16(Bits16<G>& f, uint16_t* base, size_
 #pragma unroll
         for (int k = 0; k < G; k++) {
             const unsigned v = v0 + 8 * k + 2 * q;
-            if (vec && v + 2 <= V) *reinterpret_cast<uint32_t*>(p + 8 * k) = f.h[g][k];
+            if (align >= 4 && v + 2 <= V) *reinterpret_cast<uint32_t*>(p + 8 * k) = f.h[g][k];
             else {
                 if (v < V) p[8 * k] = (uint16_t)f.h[g][k];
                 if (v + 1 < V) p[8 * k + 1] = (uint16_t)(f.h[g][k] >> 16);
@@ -310,7 +311,7 @@ __device__ __forceinline__ void store_rows16(Bits16<G>& f, uint16_t* base, size_
 }
 // The chunk transposed: 8 G lines of 32 values.  Blocks are transposed here; the lines v run over k, and the 32 rows u along a line.
 template <int G>
-__device__ __forceinline__ void store_columns16(const Bits16<G>& f, uint16_t* base, size_t ld, unsigned u0, unsigned v0, unsigned U, unsigned V, bool vec)
+__device__ __forceinline__ void store_columns16(const Bits16<G>& f, uint16_t* base, size_t ld, unsigned u0, unsigned v0, unsigned U, unsigned V, int align)
 {
     const int lane = threadIdx.x & 31, q = lane & 3;
     const unsigned v = v0 + lane / 4;
@@ -320,18 +321,54 @@ __device__ __forceinline__ void store_columns16(const Bits16<G>& f, uint16_t* ba
 #pragma unroll
         for (int g = 0; g < 4; g++) r[g] = block_transpose(f.h[g][k]);
         uint16_t* p = base + (size_t)(v + 8 * k) * ld + u0;
-        if (vec && u0 + 32 <= U) {
+        if (align == 16 && u0 + 32 <= U) {
             quad_transpose(r);
             if (v + 8 * k < V) *reinterpret_cast<uint4*>(p + 8 * q) = make_uint4(r[0], r[1], r[2], r[3]);
         } else if (v + 8 * k < V) {
 #pragma unroll
             for (int g = 0; g < 4; g++) {
                 const unsigned u = u0 + 8 * g + 2 * q;
-                if (u < U) p[8 * g + 2 * q] = (uint16_t)r[g];
-                if (u + 1 < U) p[8 * g + 2 * q + 1] = (uint16_t)(r[g] >> 16);
+                if (align >= 4 && u + 2 <= U) *reinterpret_cast<uint32_t*>(p + 8 * g + 2 * q) = r[g];
+                else {
+                    if (u < U) p[8 * g + 2 * q] = (uint16_t)r[g];
+                    if (u + 1 < U) p[8 * g + 2 * q + 1] = (uint16_t)(r[g] >> 16);
+                }
             }
         }
     }
+}
+// The counterpart: reads what store_columns16 would overwrite, as fragments of blocks that are still transposed.
+template <int G>
+__device__ __forceinline__ void load_columns16(Bits16<G>& f, const uint16_t* base, size_t ld, unsigned u0, unsigned v0, unsigned U, unsigned V, int align)
+{
+    const int lane = threadIdx.x & 31, q = lane & 3;
+    const unsigned v = v0 + lane / 4;
+#pragma unroll
+    for (int k = 0; k < G; k++) {
+        const uint16_t* p = base + (size_t)(v + 8 * k) * ld + u0 + 2 * q;
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+            const unsigned u = u0 + 8 * g + 2 * q;
+            if (v + 8 * k >= V) f.h[g][k] = 0;
+            else if (align >= 4 && u + 2 <= U) f.h[g][k] = *reinterpret_cast<const uint32_t*>(p + 8 * g);
+            else f.h[g][k] = (u < U ? p[8 * g] : 0u) | (u + 1 < U ? (uint32_t)p[8 * g + 1] << 16 : 0u);
+        }
+    }
+}
+template <int G>
+__device__ __forceinline__ void columns_to_fragments(Bits16<G>& f)
+{
+#pragma unroll
+    for (int g = 0; g < 4; g++)
+#pragma unroll
+        for (int k = 0; k < G; k++) f.h[g][k] = block_transpose(f.h[g][k]);
+}
+
+// Bytes by which lines of 16-bit elements are aligned.
+inline int line_alignment(const void* base, size_t ld, size_t stride)
+{
+    const uintptr_t a = reinterpret_cast<uintptr_t>(base) | (uintptr_t)(ld * 2) | (uintptr_t)(stride * 2);
+    return (a & 15) == 0 ? 16 : (a & 3) == 0 ? 4 : 2;
 }
 
 // ---------------------------------------------------------------------------------------------------------------------

@@ -22,6 +22,9 @@
 // The result is good to about 1e-3 and is therefore given in BF16 only.
 #include "narrow_mma.cuh"
 
+#include <algorithm>
+#include <type_traits>
+
 namespace cb200 {
 
 namespace {
@@ -31,7 +34,6 @@ using namespace narrow;
 constexpr float SX = 4096.f, SA = 256.f;                  // scales of the stored X and of the stored A, P
 constexpr double SUM_UNIT = 16777216.0;                    // sums of squares are counted in 2^-24
 constexpr double EPS = 1e-7;
-constexpr int SUM_BLOCKS = 296;
 
 typedef unsigned long long u64;
 
@@ -45,83 +47,160 @@ __device__ __forceinline__ float2 unpack(uint32_t h) { return __half22float2(*re
 
 // ---- norm and split ---------------------------------------------------------------------------------------------------
 
-// Sum of squares of one matrix of the batch, in 64 bits: block b takes lines b, b + blocks, ...
-template <typename T>
-__global__ void __launch_bounds__(256) sum_squares_kernel(const T* __restrict__ G, size_t lines, size_t len, size_t ld, size_t stride, double* __restrict__ part)
+// Eight consecutive elements, at most n of them valid.  VEC: 16-byte loads (aligned lines, a whole piece).
+template <typename T, bool VEC>
+__device__ __forceinline__ void load8(const T* p, unsigned n, float (&x)[8])
 {
+    if (VEC && n == 8) {
+        constexpr int W = 16 / sizeof(T);
+        struct alignas(16) Word { T t[W]; };
+#pragma unroll
+        for (int i = 0; i < 8 / W; i++) {
+            const Word w = reinterpret_cast<const Word*>(p)[i];
+#pragma unroll
+            for (int j = 0; j < W; j++) x[i * W + j] = to_f(w.t[j]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = i < (int)n ? to_f(p[i]) : 0.f;
+    }
+}
+
+// Sums of squares in 64 bits, one per block; the blocks of a matrix share its pieces of eight elements evenly.  Clears the sums of the
+// steps to come as well.  Bound by memory.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) sum_squares_kernel(const T* __restrict__ G, size_t lines, unsigned len, size_t ld, size_t stride,
+                                                          double* __restrict__ part, u64* __restrict__ sums, int sums_pitch)
+{
+    pdl_launch_dependents();
     const T* g = G + blockIdx.y * stride;
+    if (blockIdx.x == 0)
+        for (int i = threadIdx.x; i < sums_pitch; i += 256) sums[(size_t)blockIdx.y * sums_pitch + i] = 0;
+    const unsigned per_line = (len + 7) / 8;
+    const size_t pieces = lines * per_line, step = (size_t)gridDim.x * 256;
     double sum = 0;
-    for (size_t l = (size_t)blockIdx.x * 8 + threadIdx.x / 32; l < lines; l += (size_t)gridDim.x * 8) {
-        const T* x = g + l * ld;
-#pragma unroll 4
-        for (size_t i = threadIdx.x % 32; i < len; i += 32) {
-            const double v = to_f(x[i]);
-            sum = fma(v, v, sum);
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < pieces; i += 4 * step) {
+        float x[4][8];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const size_t at = i + k * step;
+            unsigned n = 0, c = 0;
+            size_t l = 0;
+            if (at < pieces) {
+                l = at / per_line;
+                c = (unsigned)(at - l * per_line) * 8;
+                n = min(8u, len - c);
+            }
+            load8<T, VEC>(g + l * ld + c, n, x[k]);
+        }
+        // Eight squares are added in FP32 (within 2^-21) and joined to the 64-bit sum, since a conversion for every element would take
+        // longer than the loads; pieces whose squares could leave FP32's range are converted one by one.  NaN passes either way.
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            float top = 0.f, low = 0.f;
+#pragma unroll
+            for (int j = 0; j < 8; j++) { top = fmaxf(top, fabsf(x[k][j])); low = fmaf(x[k][j], x[k][j], low); }
+            double more = low;
+            if (top > 1e18f || (top < 1e-15f && top > 0.f)) {
+                more = 0;
+                for (int j = 0; j < 8; j++) more = fma((double)x[k][j], (double)x[k][j], more);
+            }
+            sum += more;
         }
     }
-    __shared__ double sums[8];
-    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    if (threadIdx.x % 32 == 0) sums[threadIdx.x / 32] = sum;
+    double all = sum;
+    __shared__ double per_warp[8];
+    for (int d = 16; d > 0; d >>= 1) all += __shfl_xor_sync(0xffffffffu, all, d);
+    if (threadIdx.x % 32 == 0) per_warp[threadIdx.x / 32] = all;
     __syncthreads();
     if (threadIdx.x == 0) {
-        for (int w = 1; w < 8; w++) sum += sums[w];
-        part[(size_t)blockIdx.y * gridDim.x + blockIdx.x] = sum;
+        for (int w = 1; w < 8; w++) all += per_warp[w];
+        part[(size_t)blockIdx.y * gridDim.x + blockIdx.x] = all;
     }
 }
 
 // X0 = G / (|G| + eps), times SX, as hi + lo; FLIP: transposed on the way (G has more lines than elements per line).
-// A matrix that holds a NaN or an infinity becomes NaN everywhere.  64 x 64 elements per CTA.
-template <typename T, bool FLIP>
+// A matrix that holds a NaN or an infinity becomes NaN everywhere.  64 lines x 64 elements per CTA.  Bound by memory.
+template <typename T, bool VEC, bool FLIP>
 __global__ void __launch_bounds__(256) split_kernel(const T* __restrict__ G, size_t lines, size_t len, size_t ld, size_t stride, const double* __restrict__ part,
                                                     int parts, __half* __restrict__ hi, __half* __restrict__ lo, size_t ldx, size_t stride_x,
                                                     u64* __restrict__ sums, int sums_pitch, unsigned tiles_len)
 {
-    __shared__ double factor;
+    __shared__ float factors[2];
     __shared__ float tile[FLIP ? 64 : 1][65];
+    pdl_launch_dependents();
     const unsigned z = blockIdx.y;
+    const size_t l0 = (size_t)(blockIdx.x / tiles_len) * 64, i0 = (size_t)(blockIdx.x % tiles_len) * 64;
+    const T* g = G + z * stride;
+    // A thread's two pieces of eight elements: lines k and k + 32 of the tile.  (Read before the norm is known.)
+    const int piece = threadIdx.x % 8;
+    const size_t i = i0 + 8 * piece;
+    const unsigned n = i < len ? (unsigned)min((size_t)8, len - i) : 0;
+    float x[2][8];
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        const size_t l = l0 + threadIdx.x / 8 + 32 * h;
+        load8<T, VEC>(g + l * ld + i, l < lines ? n : 0, x[h]);
+    }
+    pdl_wait();
     if (threadIdx.x < 32) {
         double sum = 0;
-        for (int i = threadIdx.x; i < parts; i += 32) sum += part[(size_t)z * parts + i];
+        for (int k = threadIdx.x; k < parts; k += 32) sum += part[(size_t)z * parts + k];
         for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
         if (threadIdx.x == 0) {
+            // The factor SX / (norm + eps) may lie outside FP32: a power of two and a number in [1, 2).
             const double norm = sqrt(sum), f = 1.0 / (norm + EPS);
-            factor = isfinite(norm) ? f * SX : nan("");
+            int e;
+            const double m = frexp(f * SX, &e);
+            factors[0] = isfinite(norm) ? (float)ldexp(1.0, e - 1) : nanf("");
+            factors[1] = (float)(2.0 * m);
             if (blockIdx.x == 0) sums[(size_t)z * sums_pitch] = isfinite(norm) ? (u64)(norm * f * norm * f * SUM_UNIT) : 0;
         }
     }
     __syncthreads();
-    const double f = factor;
-    const size_t l0 = (size_t)(blockIdx.x / tiles_len) * 64, i0 = (size_t)(blockIdx.x % tiles_len) * 64;
-    const T* g = G + z * stride;
-    __half* h = hi + z * stride_x;
-    __half* w = lo + z * stride_x;
+    const float f0 = factors[0], f1 = factors[1];
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+        for (int j = 0; j < 8; j++) x[h][j] = x[h][j] * f0 * f1;
+    size_t out_line[2], out_at;
+    bool write[2];
     if (!FLIP) {
-        for (int k = threadIdx.x / 32; k < 64; k += 8) {
-            const size_t l = l0 + k, i = i0 + 2 * (threadIdx.x % 32);      // pairs: the pitch of X is even
-            if (l >= lines || i >= len) continue;
-            const float a = (float)(to_f(g[l * ld + i]) * f), b = i + 1 < len ? (float)(to_f(g[l * ld + i + 1]) * f) : 0.f;
-            const __half2 t = __floats2half2_rn(a, b);
-            const float2 r = __half22float2(t);
-            *reinterpret_cast<__half2*>(h + l * ldx + i) = t;
-            *reinterpret_cast<__half2*>(w + l * ldx + i) = __floats2half2_rn(a - r.x, b - r.y);
+        out_at = i;
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            out_line[h] = l0 + threadIdx.x / 8 + 32 * h;
+            write[h] = out_line[h] < lines && n > 0;
         }
     } else {
-        for (int k = threadIdx.x / 32; k < 64; k += 8)
-            for (int j = threadIdx.x % 32; j < 64; j += 32) {
-                const size_t l = l0 + k, i = i0 + j;
-                tile[k][j] = l < lines && i < len ? (float)(to_f(g[l * ld + i]) * f) : 0.f;
-            }
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) tile[threadIdx.x / 8 + 32 * h][8 * piece + j] = x[h][j];
         __syncthreads();
-        for (int j = threadIdx.x / 32; j < 64; j += 8) {
-            const int k = 2 * (threadIdx.x % 32);
-            const size_t l = l0 + k, i = i0 + j;
-            if (l >= lines || i >= len) continue;
-            const float a = tile[k][j], b = tile[k + 1][j];
-            const __half2 t = __floats2half2_rn(a, b);
-            const float2 r = __half22float2(t);
-            *reinterpret_cast<__half2*>(h + i * ldx + l) = t;
-            *reinterpret_cast<__half2*>(w + i * ldx + l) = __floats2half2_rn(a - r.x, b - r.y);
+        out_at = l0 + 8 * piece;
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int c = threadIdx.x / 8 + 32 * h;
+            out_line[h] = i0 + c;
+            write[h] = out_line[h] < len && out_at < lines;
+#pragma unroll
+            for (int j = 0; j < 8; j++) x[h][j] = tile[8 * piece + j][c];
         }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        if (!write[h]) continue;
+        uint32_t a[4], r[4];                               // the pitch is a multiple of 8: what lies beyond the matrix is padding
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            a[j] = pack(x[h][2 * j], x[h][2 * j + 1]);
+            const float2 t = unpack(a[j]);
+            r[j] = pack(x[h][2 * j] - t.x, x[h][2 * j + 1] - t.y);
+        }
+        const size_t at = z * stride_x + out_line[h] * ldx + out_at;
+        *reinterpret_cast<uint4*>(hi + at) = make_uint4(a[0], a[1], a[2], a[3]);
+        *reinterpret_cast<uint4*>(lo + at) = make_uint4(r[0], r[1], r[2], r[3]);
     }
 }
 
@@ -165,8 +244,8 @@ struct EpiGram {                                           // A <- X X' - t I
                 if (d == 1) b -= st.t;
                 o.h[g][k] = pack(a, b);
             }
-        if (mirror) store_columns16<G>(o, bits(A + z * stride), ld, u0, v0, s.U, s.V, true);
-        store_rows16<G>(o, bits(A + z * stride), ld, u0, v0, s.U, s.V, true);
+        if (mirror) store_columns16<G>(o, bits(A + z * stride), ld, u0, v0, s.U, s.V, 16);
+        store_rows16<G>(o, bits(A + z * stride), ld, u0, v0, s.U, s.V, 16);
     }
     __device__ void end(State&, unsigned, unsigned) const {}
 };
@@ -182,12 +261,12 @@ struct EpiSquare {                                         // P <- (b + 2 c t) A
     template <int G>
     __device__ void fetch(Pre<G>& p, const Shape& s, unsigned z, unsigned u0, unsigned v0) const
     {
-        load_rows16<G>(p.a, bits(A + z * stride), ld, u0, v0, s.U, s.V, true);
+        load_rows16<G>(p.a, bits(A + z * stride), ld, u0, v0, s.U, s.V, 16);
     }
     template <int G>
     __device__ void chunk(State& st, Pre<G>& p, const Shape& s, unsigned z, unsigned u0, unsigned v0, unsigned v_next, bool mirror, float (&x)[4][G][2]) const
     {
-        rows_to_fragments<G>(p.a, v0, s.V, true);
+        rows_to_fragments<G>(p.a, v0, s.V, 16);
         const float f = c / SA;
         Bits16<G> o;
 #pragma unroll
@@ -198,8 +277,8 @@ struct EpiSquare {                                         // P <- (b + 2 c t) A
                 o.h[g][k] = pack(fmaf(st.b, a.x, f * x[g][k][0]), fmaf(st.b, a.y, f * x[g][k][1]));
             }
         if (v_next != ~0u) fetch<G>(p, s, z, u0, v_next);
-        if (mirror) store_columns16<G>(o, bits(P + z * stride), ld, u0, v0, s.U, s.V, true);
-        store_rows16<G>(o, bits(P + z * stride), ld, u0, v0, s.U, s.V, true);
+        if (mirror) store_columns16<G>(o, bits(P + z * stride), ld, u0, v0, s.U, s.V, 16);
+        store_rows16<G>(o, bits(P + z * stride), ld, u0, v0, s.U, s.V, 16);
     }
     __device__ void end(State&, unsigned, unsigned) const {}
 };
@@ -213,8 +292,8 @@ struct UpdateTerm {
     template <int G>
     __device__ void fetch(Pre<G>& p, const Shape& s, unsigned z, unsigned u0, unsigned v0) const
     {
-        load_rows16<G>(p.h, bits(hi + z * stride), ld, u0, v0, s.U, s.V, true);
-        load_rows16<G>(p.l, bits(lo + z * stride), ld, u0, v0, s.U, s.V, true);
+        load_rows16<G>(p.h, bits(hi + z * stride), ld, u0, v0, s.U, s.V, 16);
+        load_rows16<G>(p.l, bits(lo + z * stride), ld, u0, v0, s.U, s.V, 16);
     }
     __device__ float coefficient(unsigned z) const
     {
@@ -225,8 +304,8 @@ struct UpdateTerm {
     template <int G>
     __device__ void add(Pre<G>& p, const Shape& s, unsigned v0, float coefficient, float scale, float (&x)[4][G][2]) const
     {
-        rows_to_fragments<G>(p.h, v0, s.V, true);
-        rows_to_fragments<G>(p.l, v0, s.V, true);
+        rows_to_fragments<G>(p.h, v0, s.V, 16);
+        rows_to_fragments<G>(p.l, v0, s.V, 16);
         const float f = scale * ((c == 0.f ? b : 1.f) / SA), w = scale * coefficient;
 #pragma unroll
         for (int g = 0; g < 4; g++)
@@ -276,8 +355,8 @@ struct EpiUpdate {
                 sum += in && (whole || v + 1 < s.V) ? b * b : 0.f;
             }
         st.sum += sum;
-        store_rows16<G>(h, bits(hi + z * t.stride), t.ld, u0, v0, s.U, s.V, true);
-        store_rows16<G>(l, bits(lo + z * t.stride), t.ld, u0, v0, s.U, s.V, true);
+        store_rows16<G>(h, bits(hi + z * t.stride), t.ld, u0, v0, s.U, s.V, 16);
+        store_rows16<G>(l, bits(lo + z * t.stride), t.ld, u0, v0, s.U, s.V, 16);
     }
     __device__ void end(State& st, unsigned z, unsigned) const
     {
@@ -297,13 +376,16 @@ struct EpiOut {                                            // O <- alpha X + bet
     UpdateTerm t;
     uint16_t* O; size_t ldo, stride_o;                     // BF16
     float alpha, beta;
-    bool flip, vec;                                        // flip: element (u, v) at O[v * ldo + u]; vec: 16-byte accesses of O allowed
+    bool flip;                                             // element (u, v) at O[v * ldo + u]
+    int align;                                             // of O's lines
     __device__ void begin(State& st, const Shape&, unsigned z, unsigned) const { st.a = t.coefficient(z); }
     template <int G>
     __device__ void fetch(Pre<G>& p, const Shape& s, unsigned z, unsigned u0, unsigned v0) const
     {
         t.fetch<G>(p.x, s, z, u0, v0);
-        if (beta != 0.f && !flip) load_rows16<G>(p.o, O + z * stride_o, ldo, u0, v0, s.U, s.V, vec);
+        if (beta == 0.f) return;
+        if (flip) load_columns16<G>(p.o, O + z * stride_o, ldo, u0, v0, s.U, s.V, align);
+        else load_rows16<G>(p.o, O + z * stride_o, ldo, u0, v0, s.U, s.V, align);
     }
     template <int G>
     __device__ void chunk(State& st, Pre<G>& p, const Shape& s, unsigned z, unsigned u0, unsigned v0, unsigned v_next, bool, float (&x)[4][G][2]) const
@@ -311,19 +393,8 @@ struct EpiOut {                                            // O <- alpha X + bet
         t.add<G>(p.x, s, v0, st.a, alpha / SX, x);
         uint16_t* o = O + z * stride_o;
         if (beta != 0.f) {
-            const int lane = threadIdx.x & 31;
-            if (flip) {                                    // fragments of the transposed matrix
-#pragma unroll
-                for (int g = 0; g < 4; g++)
-#pragma unroll
-                    for (int k = 0; k < G; k++) {
-                        const unsigned u = u0 + 8 * g + lane / 4, v = v0 + 8 * k + 2 * (lane & 3);
-                        const uint32_t a = u < s.U && v < s.V ? o[(size_t)v * ldo + u] : 0u, b = u < s.U && v + 1 < s.V ? o[(size_t)(v + 1) * ldo + u] : 0u;
-                        p.o.h[g][k] = a | b << 16;
-                    }
-            } else {
-                rows_to_fragments<G>(p.o, v0, s.V, vec);
-            }
+            if (flip) columns_to_fragments<G>(p.o);
+            else rows_to_fragments<G>(p.o, v0, s.V, align);
 #pragma unroll
             for (int g = 0; g < 4; g++)
 #pragma unroll
@@ -342,13 +413,29 @@ struct EpiOut {                                            // O <- alpha X + bet
                 const __nv_bfloat162 b = __floats2bfloat162_rn(x[g][k][0], x[g][k][1]);
                 r.h[g][k] = *reinterpret_cast<const uint32_t*>(&b);
             }
-        if (flip) store_columns16<G>(r, o, ldo, u0, v0, s.U, s.V, vec);
-        else store_rows16<G>(r, o, ldo, u0, v0, s.U, s.V, vec);
+        if (flip) store_columns16<G>(r, o, ldo, u0, v0, s.U, s.V, align);
+        else store_rows16<G>(r, o, ldo, u0, v0, s.U, s.V, align);
     }
     __device__ void end(State&, unsigned, unsigned) const {}
 };
 
 // ---- the chain ----------------------------------------------------------------------------------------------------------
+
+// A plain kernel as a link of the chain: it may start while the one before it drains and waits in pdl_wait().
+template <typename... KArgs, typename... Args>
+cudaError_t launch_chained(void (*kernel)(KArgs...), dim3 grid, unsigned block, cudaStream_t s, Args... args)
+{
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(block);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
 
 template <typename T>
 cudaError_t orthogonalize_typed(const OrthProblem& p, cudaStream_t s)
@@ -359,7 +446,9 @@ cudaError_t orthogonalize_typed(const OrthProblem& p, cudaStream_t s)
     auto up = [](size_t v, size_t q) { return (v + q - 1) / q * q; };
     const size_t ldx = up(m, 8), ldn = up(n, 8), xs = n * ldx, as = n * ldn;
     const int pitch = p.steps + 1;
-    const size_t lines_blocks = (p.lines + 7) / 8, parts = lines_blocks < SUM_BLOCKS ? lines_blocks : SUM_BLOCKS;
+    // Blocks of the norm: about 8 pieces a thread, at most two blocks per SM over the batch.
+    const size_t blocks = (p.lines * ((p.len + 7) / 8) + 2047) / 2048, most = std::max<size_t>(1, 2 * (size_t)sm_count() / batch);
+    const size_t parts = std::min(blocks, most);
     // workspace: hi (two of them, read and written in turn), lo, A, P, sums of squares, partial norms
     const size_t x_bytes = up(batch * xs * 2, 256), a_bytes = up(batch * as * 2, 256), sum_bytes = up(batch * pitch * 8, 256);
     unsigned char* ws = nullptr;
@@ -373,17 +462,19 @@ cudaError_t orthogonalize_typed(const OrthProblem& p, cudaStream_t s)
     double* part = reinterpret_cast<double*>(ws + 3 * x_bytes + 2 * a_bytes + sum_bytes);
     const T* G = static_cast<const T*>(p.G) + p.offG;
 
-    e = cudaMemsetAsync(sums, 0, batch * pitch * 8, s);
+    const size_t tl = (p.len + 63) / 64, tiles = tl * ((p.lines + 63) / 64);
+    if (tiles >= (1u << 31)) e = cudaErrorNotSupported;
     if (e == cudaSuccess) {
-        sum_squares_kernel<T><<<dim3((unsigned)parts, (unsigned)batch), 256, 0, s>>>(G, p.lines, p.len, p.ldg, p.strideG, part);
-        const size_t tl = (p.len + 63) / 64, tiles = tl * ((p.lines + 63) / 64);
-        if (tiles >= (1u << 31)) e = cudaErrorNotSupported;
-        else if (flip)
-            split_kernel<T, true><<<dim3((unsigned)tiles, (unsigned)batch), 256, 0, s>>>(G, p.lines, p.len, p.ldg, p.strideG, part, (int)parts, hi[0], lo, ldx, xs, sums, pitch, (unsigned)tl);
-        else
-            split_kernel<T, false><<<dim3((unsigned)tiles, (unsigned)batch), 256, 0, s>>>(G, p.lines, p.len, p.ldg, p.strideG, part, (int)parts, hi[0], lo, ldx, xs, sums, pitch, (unsigned)tl);
-        count_launch(2);
-        if (e == cudaSuccess) e = cudaGetLastError();
+        const bool vec = aligned16(G) && p.ldg * sizeof(T) % 16 == 0 && (batch == 1 || p.strideG * sizeof(T) % 16 == 0);
+        const dim3 g1((unsigned)parts, (unsigned)batch), g2((unsigned)tiles, (unsigned)batch);
+        auto prepare = [&](auto is_vec, auto is_flip) {
+            constexpr bool V = decltype(is_vec)::value, F = decltype(is_flip)::value;
+            sum_squares_kernel<T, V><<<g1, 256, 0, s>>>(G, p.lines, (unsigned)p.len, p.ldg, p.strideG, part, sums, pitch);
+            count_launch(2);
+            return launch_chained(split_kernel<T, V, F>, g2, 256, s, G, p.lines, p.len, p.ldg, p.strideG, (const double*)part, (int)parts, hi[0], lo, ldx, xs, sums, pitch, (unsigned)tl);
+        };
+        if (vec) e = flip ? prepare(std::true_type{}, std::true_type{}) : prepare(std::true_type{}, std::false_type{});
+        else     e = flip ? prepare(std::false_type{}, std::true_type{}) : prepare(std::false_type{}, std::false_type{});
     }
     const float inv_n = 1.f / (float)n;
     for (int k = 0; k < p.steps && e == cudaSuccess; k++) {
@@ -405,8 +496,8 @@ cudaError_t orthogonalize_typed(const OrthProblem& p, cudaStream_t s)
             e = run_planned<KIND_F16, true>(c != 0.f ? op : oa, ox, up_, EpiUpdate{t, hi[(k + 1) & 1], lo, sums + k + 1}, s);
         } else {
             uint16_t* O = static_cast<uint16_t*>(p.O) + p.offO;
-            const bool vec = aligned16(O) && p.ldo % 8 == 0 && (batch == 1 || p.strideO % 8 == 0);
-            e = run_planned<KIND_F16, true>(c != 0.f ? op : oa, ox, up_, EpiOut{t, O, p.ldo, p.strideO, p.alpha, p.beta, flip, vec}, s);
+            const int align = line_alignment(O, p.ldo, batch > 1 ? p.strideO : 0);
+            e = run_planned<KIND_F16, true>(c != 0.f ? op : oa, ox, up_, EpiOut{t, O, p.ldo, p.strideO, p.alpha, p.beta, flip, align}, s);
         }
     }
     const cudaError_t e2 = ws_free(ws, s);
