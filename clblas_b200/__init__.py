@@ -261,7 +261,12 @@ def _handle_array(items: Optional[Sequence], default_current_stream: bool = Fals
     return len(items), arr
 
 
+_ONE_HANDLE = ctypes.c_void_p * 1
+
+
 def _queues_events(queues, wait, events):
+    if queues is None and wait is None and events is None:        # the common call: current stream, no events
+        return 1, _ONE_HANDLE(_current_stream()), 0, None, None
     nq, q = _handle_array(queues, default_current_stream=True)
     nw, w = _handle_array(wait)
     _, e = _handle_array(events)

@@ -35,7 +35,7 @@ template <> __device__ __forceinline__ float2 unpack16<__nv_bfloat16>(uint32_t h
 // C[u, v] <- alpha su[u] sv[v] acc + beta C[u, v].
 template <typename T>
 struct EpiScaled {
-    static constexpr bool kChained = false;
+    static constexpr bool kChained = false, kHeavy = sizeof(T) == 4;
     struct State { float factor[4]; };
     template <int G> struct Pre { Bits16<G> c; };
     const float* su;                // scales of the rows u and the columns v; nullptr: ones
@@ -60,7 +60,7 @@ struct EpiScaled {
         else load_rows16<G>(p.c, reinterpret_cast<const uint16_t*>(C), ld, u0, v0, s.U, s.V, align);
     }
     template <int G>
-    __device__ void chunk(State& st, Pre<G>& p, const Shape& s, unsigned z, unsigned u0, unsigned v0, unsigned v_next, bool, float (&x)[4][G][2]) const
+    __device__ void chunk(State& st, Pre<G>& p, const Shape& s, unsigned z, unsigned u0, unsigned v0, unsigned v_next, int, float (&x)[4][G][2]) const
     {
         const int lane = threadIdx.x & 31, q = lane & 3;
         const unsigned u = u0 + lane / 4;
@@ -241,10 +241,11 @@ cudaError_t multiply(const Operand& lines, const Operand& len, const float* s_li
         s.U = (unsigned)L; s.V = (unsigned)W;
         return EpiScaled<T>{s_lines, s_len, alpha, beta, C, ldc, false, align};
     };
+    // Few columns: k over as many CTAs as the machine has room for, two slabs each at least.
     auto split_for = [&](unsigned bn, unsigned per_sm) {
         const size_t tiles = ((s.U + BM - 1) / BM) * (size_t)((s.V + bn - 1) / bn);
         unsigned split = 1;
-        while (split < 8 && tiles * split * 2 <= (size_t)sms * per_sm && split * 2 * 2 <= nk) split *= 2;
+        while (split < (bn == 128 ? 4u : 8u) && tiles * split * 2 <= (size_t)sms * per_sm && split * 2 * 2 <= nk) split *= 2;
         return split;
     };
     if (L <= 128 && W > L) {

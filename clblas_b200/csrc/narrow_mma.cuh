@@ -51,10 +51,12 @@ __device__ __forceinline__ uint32_t cluster_nctarank()
     return r;
 }
 // All threads of all CTAs of the cluster; the warp must be converged.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_sync()
 {
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    cluster_arrive();
+    cluster_wait();
 }
 // Address of `saddr` (this CTA's shared memory) in the shared memory of CTA `rank` of the cluster.
 __device__ __forceinline__ uint32_t map_shared(uint32_t saddr, uint32_t rank)
@@ -179,20 +181,32 @@ __device__ __forceinline__ float acc_value(uint32_t v) { return KIND == KIND_I8 
 struct Shape {
     unsigned U, V, K, batch;
     unsigned tilesU, tilesV, tiles;           // tiles: per batch entry (of the lower triangle when tri)
-    int tri;                                  // 1: U == V, square tiles, only tiles with tu >= tv; the functor mirrors them
+    int tri;                                  // 1: U == V, symmetric: tiles that touch the lower triangle only (in blocks of 128 x 128)
+    unsigned per;                             // tri: columns of tiles per row of tiles (tile height / tile width, 1 or 2)
 };
+
+// What becomes of a chunk: its 128 x 128 block lies below the diagonal (stored at both places), on it, or above (a tile that
+// straddles the diagonal; not stored).
+enum Part { PART_PLAIN = 0, PART_BELOW = 1, PART_ABOVE = -1 };
+__device__ __forceinline__ int part_of(const Shape& s, unsigned u0, unsigned v0)
+{
+    if (!s.tri) return PART_PLAIN;
+    const unsigned bu = u0 / 128, bv = v0 / 128;
+    return bu > bv ? PART_BELOW : bu < bv ? PART_ABOVE : PART_PLAIN;
+}
 
 // Tile number -> (tu, tv).  Full: groups of GROUP rows of tiles, column by column inside a group, so that the tiles in flight
 // share operands in L2.  Triangle: row by row.
 constexpr unsigned GROUP = 8;
 __host__ __device__ inline void tile_coords(const Shape& s, unsigned t, unsigned& tu, unsigned& tv)
 {
-    if (s.tri) {
-        unsigned r = (unsigned)((sqrtf(8.0f * (float)t + 1.0f) - 1.0f) * 0.5f);
-        while (r * (r + 1) / 2 > t) r--;
-        while ((r + 1) * (r + 2) / 2 <= t) r++;
+    if (s.tri) {                              // row r has per * (r + 1) tiles
+        const unsigned p = t / s.per;
+        unsigned r = (unsigned)((sqrtf(8.0f * (float)p + 1.0f) - 1.0f) * 0.5f);
+        while (r * (r + 1) / 2 > p) r--;
+        while ((r + 1) * (r + 2) / 2 <= p) r++;
         tu = r;
-        tv = t - r * (r + 1) / 2;
+        tv = t - s.per * (r * (r + 1) / 2);
         return;
     }
     const unsigned per_group = GROUP * s.tilesV, g = t / per_group, first = g * GROUP, left = s.tilesU - first;
@@ -204,11 +218,11 @@ __host__ __device__ inline void tile_coords(const Shape& s, unsigned t, unsigned
 // ---------------------------------------------------------------------------------------------------------------------
 // Epilogue.  A warp finishes chunks of 32 rows x 8 G columns, held as fragments x[g][k][e]: row 8 g + lane / 4, column
 // 8 k + 2 (lane % 4) + e.  What a functor has:
-//   kChained      launched as a link of a chain of products (programmatic dependent launch)
+//   kChained      a link of a chain of products: its successor may start as soon as all its CTAs have
+//   kHeavy        reads as much as it writes (for choose_plan)
 //   begin()       per thread and tile
 //   Pre, fetch()  what a chunk needs besides the accumulators, requested one chunk ahead
-//   chunk()       computes and stores; requests the next chunk's (at column v_next, ~0u: none) as soon as its own is used; mirror: the
-//                 result is symmetric and the tile off its diagonal, so it is stored at (v, u) too
+//   chunk()       computes and stores (where: part_of()); requests the next chunk's (at column v_next, ~0u: none) as soon as its own is used
 //   end()         per thread and tile
 //
 // Nothing goes through shared memory: its bandwidth is what the products and the loads that feed them use up (both sides
@@ -439,7 +453,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 narrow_persistent_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__ CUtensorMap mapQ, const Shape s, const Epi epi)
 {
     constexpr int STAGES = persistent_stages<BN, CG>(), STAGE = stage_bytes<BN, CG>();
-    constexpr uint32_t TMEM_COLS = 2 * BN < 32 ? 32 : 2 * BN;
+    constexpr uint32_t TMEM_COLS = 2 * BN > 256 ? 512 : 256;          // two accumulators; a power of two
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE);
@@ -473,7 +487,7 @@ narrow_persistent_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_
     if (CG == 2) cluster_sync();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    pdl_launch_dependents();
+    if (Epi::kChained) pdl_launch_dependents();
     pdl_wait();
 
     if (warp == 0) {
@@ -543,7 +557,7 @@ narrow_persistent_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_
                         else mbar_arrive(&acc_empty[a]);
                     }
                 }
-                epi.chunk(st, pre, s, z, u0, v0 + c * 32, c + 1 < CHUNKS ? v0 + (c + 1) * 32 : ~0u, s.tri && tu != tv, x);
+                epi.chunk(st, pre, s, z, u0, v0 + c * 32, c + 1 < CHUNKS ? v0 + (c + 1) * 32 : ~0u, part_of(s, u0, v0 + c * 32), x);
             }
             epi.end(st, z, t);
         }
@@ -561,26 +575,28 @@ narrow_persistent_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_
 // ---------------------------------------------------------------------------------------------------------------------
 
 // Two CTAs per SM for the narrow tiles (decoding: the loads of one run under the start and the end of the other), one for BN = 128.
-template <int BN>
-constexpr int split_stages() { return BN == 32 ? 5 : BN == 64 ? 4 : 6; }
-template <int BN>
-constexpr int split_smem() { return split_stages<BN>() * stage_bytes<BN, 1>() + 1024 + 256; }
+// The partial sums have a place of their own beside the ring, so that a CTA may receive them while its products still run.
+template <int BN, int S>
+constexpr int split_part() { return S == 1 ? 0 : BN * BM * 4 * (S > BN / 8 ? S * 8 / BN : 1); }
+template <int BN, int S>
+constexpr int split_stages() { return BN == 128 ? (S == 1 ? 6 : 4) : ((232448 - 2048) / 2 - 1280 - split_part<BN, S>()) / stage_bytes<BN, 1>(); }
+template <int BN, int S>
+constexpr int split_smem() { return split_stages<BN, S>() * stage_bytes<BN, 1>() + split_part<BN, S>() + 1024 + 256; }
 
 template <int KIND, int BN, int S, bool QMN, class Epi>
 __global__ void __launch_bounds__(THREADS)
 narrow_split_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__ CUtensorMap mapQ, const Shape s, const Epi epi)
 {
-    constexpr int STAGES = split_stages<BN>(), STAGE = stage_bytes<BN, 1>();
+    constexpr int STAGES = split_stages<BN, S>(), STAGE = stage_bytes<BN, 1>();
     constexpr uint32_t TMEM_COLS = BN;
     // Column groups of 8 that a rank sums and finishes; with S > BN / 8 the last ranks have none.
     constexpr int GROUPS = BN / 8, OWNERS = S < GROUPS ? S : GROUPS, OWN = GROUPS / OWNERS;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    // The ring is free once the products of every CTA of the cluster are done: the partial sums use it again, as fragments:
-    // [S ranks][4 quarters][OWN groups][4 g][32 lanes] pairs.
-    uint2* part = reinterpret_cast<uint2*>(smem);
-    static_assert(S * OWN * 8 * BM * 4 <= STAGES * STAGE, "the ring holds the partial sums");
-    uint64_t* full = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE);
+    // Partial sums as fragments: [S ranks][4 quarters][OWN groups][4 g][32 lanes] pairs.
+    uint2* part = reinterpret_cast<uint2*>(smem + STAGES * STAGE);
+    static_assert(S == 1 || S * OWN * 8 * BM * 4 == split_part<BN, S>(), "size of the partial sums");
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE + split_part<BN, S>());
     uint64_t* empty = full + STAGES;
     uint64_t* acc_full = empty + STAGES;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
@@ -603,12 +619,14 @@ narrow_split_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_const
         tma_prefetch_descriptor(&mapP);
         tma_prefetch_descriptor(&mapQ);
     }
+    __syncwarp();
+    if (S > 1) cluster_arrive();                                  // waited for before this CTA writes to the others: by then they run
     if (warp == 1) tmem_alloc<1>(tmem_slot, TMEM_COLS);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    pdl_launch_dependents();
+    if (Epi::kChained) pdl_launch_dependents();
     pdl_wait();
 
     if (warp == 0) {
@@ -634,26 +652,30 @@ narrow_split_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_const
     }
     const int quarter = warp & 3, half = (warp - 2) / 4;
     const unsigned u0 = tu * BM + quarter * 32;
-    const bool mirror = s.tri && tu != tv;
+    const int where = part_of(s, u0, tv * BN);
     typename Epi::State st;
+    // The columns this warp finishes: chunks of G groups, every second one (the two warps of a quarter take turns).
+    constexpr int G = OWN < 4 ? OWN : 4;
+    const unsigned v_own = tv * BN + rank * (OWN * 8) + half * (G * 8);
+    const bool finishes = warp >= 2 && rank < OWNERS && half < OWN / G;
+    typename Epi::template Pre<G> pre;
     bool ok = true;
     if (warp >= 2) {
         epi.begin(st, s, z, u0);
+        if (finishes) epi.fetch(pre, s, z, u0, v_own);
         ok = __all_sync(0xffffffffu, mbar_wait(acc_full, 0));
         tc_fence_after();
     }
     __syncwarp();
-    if (S > 1) cluster_sync();                                    // the products of all CTAs of the cluster are done
+    if (S > 1) cluster_wait();
     if (warp >= 2 && ok) {
 #pragma unroll 1
         for (int c = half; c < BN / 32; c += 2) {
-            typename Epi::template Pre<4> pre;
-            if (S == 1) epi.fetch(pre, s, z, u0, tv * BN + c * 32);
             const uint32_t taddr = tmem + ((uint32_t)(32 * quarter) << 16) + c * 32;
-            if (S == 1) {
+            if constexpr (S == 1) {
                 float x[4][4][2];
                 read_chunk<KIND>(x, taddr);
-                epi.chunk(st, pre, s, z, u0, tv * BN + c * 32, ~0u, mirror, x);
+                epi.chunk(st, pre, s, z, u0, tv * BN + c * 32, c + 2 < BN / 32 ? tv * BN + (c + 2) * 32 : ~0u, where, x);
             } else {
                 uint32_t a[16], b[16];
                 __syncwarp();
@@ -675,13 +697,10 @@ narrow_split_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_const
     if (S > 1) {
         __syncwarp();
         cluster_sync();
-        if (warp >= 2 && ok && rank < OWNERS) {
-            constexpr int G = OWN < 4 ? OWN : 4;                  // groups per chunk; the two warps of a quarter take turns
+        if (finishes && ok) {
 #pragma unroll 1
             for (int c = half; c < OWN / G; c += 2) {
                 const unsigned v0 = tv * BN + rank * (OWN * 8) + c * (G * 8);
-                typename Epi::template Pre<G> pre;
-                epi.fetch(pre, s, z, u0, v0);
                 float x[4][G][2];
 #pragma unroll
                 for (int k = 0; k < G; k++)
@@ -700,7 +719,7 @@ narrow_split_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_const
                             x[g][k][0] = f0; x[g][k][1] = f1;
                         }
                     }
-                epi.chunk(st, pre, s, z, u0, v0, ~0u, mirror, x);
+                epi.chunk(st, pre, s, z, u0, v0, c + 2 < OWN / G ? v0 + 2 * G * 8 : ~0u, where, x);
             }
         }
     }
@@ -741,7 +760,8 @@ inline void set_tiles(Shape& s, unsigned bu, unsigned bv)
 {
     s.tilesU = (s.U + bu - 1) / bu;
     s.tilesV = (s.V + bv - 1) / bv;
-    s.tiles = s.tri ? s.tilesU * (s.tilesU + 1) / 2 : s.tilesU * s.tilesV;
+    s.per = bu / bv;
+    s.tiles = s.tri ? s.per * (s.tilesU * (s.tilesU + 1) / 2) : s.tilesU * s.tilesV;
 }
 
 template <typename Kernel, typename Epi>
@@ -757,12 +777,12 @@ cudaError_t launch(Kernel kernel, unsigned grid, unsigned cluster, int smem, cud
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = cluster;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    // chained: the kernel before it on the stream is one of a chain of short products; it may start (barriers, tensor memory,
-    // descriptors) while that one drains, and waits for its results in pdl_wait().
+    // The kernel may start (barriers, tensor memory, descriptors) while the one before it on the stream drains, and waits for it
+    // in pdl_wait(); links of a chain let their successor do so from their own start on (kChained).
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = Epi::kChained ? 2 : 1;
+    cfg.numAttrs = 2;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, mp, mq, s, epi);
     if (e == cudaSuccess) count_launch();
     return e;
@@ -789,7 +809,7 @@ template <int KIND, int BN, int S, bool QMN, class Epi>
 cudaError_t run_split(const Operand& p, const Operand& q, Shape s, const Epi& epi, cudaStream_t st)
 {
     auto kernel = narrow_split_kernel<KIND, BN, S, QMN, Epi>;
-    constexpr int smem = split_smem<BN>();
+    constexpr int smem = split_smem<BN, S>();
     static DeviceOnce once;
     cudaError_t e = once.run([&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); });
     if (e != cudaSuccess) return e;
@@ -801,44 +821,49 @@ cudaError_t run_split(const Operand& p, const Operand& q, Shape s, const Epi& ep
     return launch(kernel, s.tiles * s.batch * S, S, smem, st, mp, mq, s, epi);
 }
 
-// How a product of more than 64 columns runs.  Estimated clocks, fitted to measurements: rounds of tiles times slabs and epilogues.
-// Operands come from L2, which gives a slab of 128 x 128 tiles every 570 clocks (32 KB per SM) and one of 256 x 256 tiles every 650
-// (32 KB per SM for twice the products) when all SMs ask at once; a lone tile gets a slab in about 300.
-//   pairs:  256 x 256 tiles on pairs of CTAs
-//   single: 128 x 128 tiles, persistent
-//   split:  128 x 128 tiles, k (and the epilogue's columns) over S CTAs of a cluster
-struct Plan { bool pairs; unsigned split; };         // split == 0: persistent
-inline Plan choose_plan(unsigned U, unsigned V, unsigned K, unsigned batch, int tri, int kind)
+// How a product of more than 64 columns runs:
+//   pairs:  256 x pairs tiles (256, 192 or 128 wide) on pairs of CTAs, persistent; 192 for 8-bit operands only (v-contiguous ones
+//           come in blocks of 64 per CTA, triangles in blocks of 128)
+//   split:  128 x 128 tiles, one per cluster of `split` CTAs, which share k and the epilogue's columns
+// The plan with the shortest estimate is taken.  The estimates, in us, are fitted to all plans measured on twelve shapes from
+// 100 x 130 to 2048 x 8192 (the best plan found for all but two, where it lost 4 and 7 %):
+//   a launch and its end                 3, persistent 5
+//   a slab of k, 128 x 128 tiles         0.30                            1 round of 136 tiles, 128 slabs: 46.7
+//   a slab of k, 256 x 256               0.30 for a lone tile, 0.37 with all SMs at it, 0.36 to 0.45 in later rounds, when
+//                                        the epilogues (0.45: `heavy` ones, that read as much as they write) share L2 with the loads
+//   a slab of k, 256 x 128               0.30, later 0.37
+//   an epilogue                          128 x 128: 5.0, 4.6, 4.2 with 1, 2, 4 CTAs at it (heavy: 6.3, 5.6, 4.5); 256 x 256: 5.0 (7.7), 256 x 128: 5.0 (7.0)
+// A round of a persistent kernel takes the longer of its slabs and the epilogue before; clusters of 4 fill 128 SMs, clusters of 8 (never the
+// best here) fewer.
+struct Plan { unsigned pairs, split; };               // one of the two is 0
+inline Plan choose_plan(unsigned U, unsigned V, unsigned K, unsigned batch, int tri, int kind, bool heavy)
 {
-    const unsigned sms = (unsigned)sm_count(), nk = (K + slab_k(kind) - 1) / slab_k(kind);
-    auto tiles = [&](unsigned b) {
-        const unsigned long long tu = (U + b - 1) / b, tv = (V + b - 1) / b;
-        return (double)(batch * (tri ? tu * (tu + 1) / 2 : tu * tv));
+    const unsigned nk = (K + slab_k(kind) - 1) / slab_k(kind);
+    const double sms = sm_count();
+    auto tiles = [&](unsigned bu, unsigned bv) {
+        const double tu = (U + bu - 1) / bu, tv = (V + bv - 1) / bv;
+        return batch * (tri ? (double)(bu / bv) * tu * (tu + 1) / 2 : tu * tv);
     };
-    const double t128 = tiles(128), t256 = tiles(256);
-    auto slab = [&](double busy, double all) { const double f = busy / sms; return 300 + (all - 300) * (f < 1 ? f : 1); };
-    auto loop = [](double per_tile, double epilogue, double rounds) {     // persistent: the epilogue runs under the next tile's slabs
-        const double longer = per_tile > epilogue ? per_tile : epilogue;
-        return per_tile + (rounds - 1) * longer + epilogue;
-    };
-    const double epi = tri ? 1500 : 1200;                                 // per chunk of 32 columns and warp
-    Plan best{true, 0};
-    double least = loop(nk * slab(2 * t256, 650), 4 * epi, std::ceil(t256 / (sms / 2))) + 2000;
-    const double single = loop(nk * slab(t128, 570), 2 * epi, std::ceil(t128 / sms)) + 1500;
-    if (single < least) { least = single; best = {false, 0}; }
-    for (unsigned s = 1; s <= 8 && s <= nk; s *= 2) {
-        const double chunks = s <= 2 ? 2.0 / s : 1;
-        const double c = std::ceil(t128 * s / sms) * (((nk + s - 1) / s) * slab(t128 * s, 570) + chunks * epi + 1500 + (s > 1 ? 1500 : 0));
-        if (c < least) { least = c; best = {false, s}; }
-    }
+    Plan best{};
+    double least = 1e30;
+    auto consider = [&](Plan plan, double us) { if (us < least) { least = us; best = plan; } };
+    const double pairs = std::floor(sms / 2), t256 = tiles(256, 256), t128 = tiles(128, 128), e256 = heavy ? 7.7 : 5.0, e128 = heavy ? 7.0 : 5.0;
+    consider({256, 0}, 5 + nk * (0.30 + 0.07 * std::fmin(1.0, t256 / pairs)) + e256 + (std::ceil(t256 / pairs) - 1) * std::fmax(nk * (heavy ? 0.45 : 0.36), e256));
+    consider({128, 0}, 5 + nk * 0.30 + 0.7 * e128 + (std::ceil(tiles(256, 128) / pairs) - 1) * std::fmax(nk * 0.37, e128));
+    if (kind == KIND_I8)
+        consider({192, 0}, 5 + nk * 0.33 + 0.75 * e256 + 0.5 + (std::ceil(tiles(256, 192) / pairs) - 1) * std::fmax(nk * (heavy ? 0.40 : 0.33), 0.75 * e256 + 0.5));
+    const double finish[3] = {heavy ? 6.3 : 5.0, heavy ? 5.6 : 4.6, heavy ? 4.5 : 4.2};
+    for (unsigned i = 0, s = 1; i < 3 && s <= nk; i++, s *= 2)
+        consider({0, s}, 3 + std::ceil(t128 * s / (s == 4 ? sms - 20 : sms)) * ((nk + s - 1) / s * 0.30 + finish[i]));
     return best;
 }
 
 template <int KIND, int BN, bool QMN, class Epi>
 cudaError_t run_split_by(unsigned split, const Operand& p, const Operand& q, const Shape& s, const Epi& epi, cudaStream_t st)
 {
+    if constexpr (BN < 128)
+        if (split == 8) return run_split<KIND, BN, 8, QMN, Epi>(p, q, s, epi, st);
     switch (split) {
-        case 8: return run_split<KIND, BN, 8, QMN, Epi>(p, q, s, epi, st);
         case 4: return run_split<KIND, BN, 4, QMN, Epi>(p, q, s, epi, st);
         case 2: return run_split<KIND, BN, 2, QMN, Epi>(p, q, s, epi, st);
         default: return run_split<KIND, BN, 1, QMN, Epi>(p, q, s, epi, st);
@@ -848,9 +873,11 @@ cudaError_t run_split_by(unsigned split, const Operand& p, const Operand& q, con
 template <int KIND, bool QMN, class Epi>
 cudaError_t run_planned(const Operand& p, const Operand& q, const Shape& s, const Epi& epi, cudaStream_t st)
 {
-    const Plan plan = choose_plan(s.U, s.V, s.K, s.batch, s.tri, KIND);
-    if (plan.pairs) return run_persistent<KIND, 256, 2, QMN, Epi>(p, q, s, epi, st);
-    if (plan.split == 0) return run_persistent<KIND, 128, 1, QMN, Epi>(p, q, s, epi, st);
+    const Plan plan = choose_plan(s.U, s.V, s.K, s.batch, s.tri, KIND, Epi::kHeavy);
+    if (plan.pairs == 256) return run_persistent<KIND, 256, 2, QMN, Epi>(p, q, s, epi, st);
+    if (plan.pairs == 128) return run_persistent<KIND, 128, 2, QMN, Epi>(p, q, s, epi, st);
+    if constexpr (KIND == KIND_I8)
+        if (plan.pairs == 192) return run_persistent<KIND, 192, 2, QMN, Epi>(p, q, s, epi, st);
     return run_split_by<KIND, 128, QMN, Epi>(plan.split, p, q, s, epi, st);
 }
 

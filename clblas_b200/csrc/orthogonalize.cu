@@ -76,22 +76,21 @@ __global__ void __launch_bounds__(256) sum_squares_kernel(const T* __restrict__ 
     const T* g = G + blockIdx.y * stride;
     if (blockIdx.x == 0)
         for (int i = threadIdx.x; i < sums_pitch; i += 256) sums[(size_t)blockIdx.y * sums_pitch + i] = 0;
-    const unsigned per_line = (len + 7) / 8;
-    const size_t pieces = lines * per_line, step = (size_t)gridDim.x * 256;
+    // Pieces of eight elements in the order of the matrix, the grid's threads apart; (line, piece of the line) is stepped by
+    // (step / per_line, step % per_line), since a 64-bit division for every piece would bound the kernel.
+    const unsigned per_line = (len + 7) / 8, step = gridDim.x * 256, at = blockIdx.x * 256 + threadIdx.x;
+    const unsigned dl = step / per_line, dc = step % per_line;
+    size_t l = at / per_line;
+    unsigned c = at % per_line;
     double sum = 0;
-    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < pieces; i += 4 * step) {
+    while (l < lines) {
         float x[4][8];
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-            const size_t at = i + k * step;
-            unsigned n = 0, c = 0;
-            size_t l = 0;
-            if (at < pieces) {
-                l = at / per_line;
-                c = (unsigned)(at - l * per_line) * 8;
-                n = min(8u, len - c);
-            }
-            load8<T, VEC>(g + l * ld + c, n, x[k]);
+            load8<T, VEC>(g + l * ld + 8 * (size_t)c, l < lines ? min(8u, len - 8 * c) : 0, x[k]);
+            l += dl;
+            c += dc;
+            if (c >= per_line) { c -= per_line; l++; }
         }
         // Eight squares are added in FP32 (within 2^-21) and joined to the 64-bit sum, since a conversion for every element would take
         // longer than the loads; pieces whose squares could leave FP32's range are converted one by one.  NaN passes either way.
@@ -220,7 +219,7 @@ __device__ __forceinline__ uint16_t* bits(__half* p) { return reinterpret_cast<u
 __device__ __forceinline__ const uint16_t* bits(const __half* p) { return reinterpret_cast<const uint16_t*>(p); }
 
 struct EpiGram {                                           // A <- X X' - t I
-    static constexpr bool kChained = true;
+    static constexpr bool kChained = true, kHeavy = false;
     struct State { float t; };
     template <int G> struct Pre {};
     __half* A; size_t ld, stride;
@@ -229,7 +228,7 @@ struct EpiGram {                                           // A <- X X' - t I
     __device__ void begin(State& st, const Shape&, unsigned z, unsigned) const { st.t = SA * shift_of(sums, (size_t)z * pitch, inv_n); }
     template <int G> __device__ void fetch(Pre<G>&, const Shape&, unsigned, unsigned, unsigned) const {}
     template <int G>
-    __device__ void chunk(State& st, Pre<G>&, const Shape& s, unsigned z, unsigned u0, unsigned v0, unsigned, bool mirror, float (&x)[4][G][2]) const
+    __device__ void chunk(State& st, Pre<G>&, const Shape& s, unsigned z, unsigned u0, unsigned v0, unsigned, int where, float (&x)[4][G][2]) const
     {
         const int lane = threadIdx.x & 31;
         const int off = (int)(u0 + lane / 4) - (int)(v0 + 2 * (lane & 3));      // row - column of x[0][0][0]
@@ -244,14 +243,14 @@ struct EpiGram {                                           // A <- X X' - t I
                 if (d == 1) b -= st.t;
                 o.h[g][k] = pack(a, b);
             }
-        if (mirror) store_columns16<G>(o, bits(A + z * stride), ld, u0, v0, s.U, s.V, 16);
-        store_rows16<G>(o, bits(A + z * stride), ld, u0, v0, s.U, s.V, 16);
+        if (where == PART_BELOW) store_columns16<G>(o, bits(A + z * stride), ld, u0, v0, s.U, s.V, 16);
+        if (where != PART_ABOVE) store_rows16<G>(o, bits(A + z * stride), ld, u0, v0, s.U, s.V, 16);
     }
     __device__ void end(State&, unsigned, unsigned) const {}
 };
 
 struct EpiSquare {                                         // P <- (b + 2 c t) A + c A^2
-    static constexpr bool kChained = true;
+    static constexpr bool kChained = true, kHeavy = false;
     struct State { float b; };
     template <int G> struct Pre { Bits16<G> a; };
     const __half* A; __half* P; size_t ld, stride;
@@ -264,7 +263,7 @@ struct EpiSquare {                                         // P <- (b + 2 c t) A
         load_rows16<G>(p.a, bits(A + z * stride), ld, u0, v0, s.U, s.V, 16);
     }
     template <int G>
-    __device__ void chunk(State& st, Pre<G>& p, const Shape& s, unsigned z, unsigned u0, unsigned v0, unsigned v_next, bool mirror, float (&x)[4][G][2]) const
+    __device__ void chunk(State& st, Pre<G>& p, const Shape& s, unsigned z, unsigned u0, unsigned v0, unsigned v_next, int where, float (&x)[4][G][2]) const
     {
         rows_to_fragments<G>(p.a, v0, s.V, 16);
         const float f = c / SA;
@@ -277,8 +276,8 @@ struct EpiSquare {                                         // P <- (b + 2 c t) A
                 o.h[g][k] = pack(fmaf(st.b, a.x, f * x[g][k][0]), fmaf(st.b, a.y, f * x[g][k][1]));
             }
         if (v_next != ~0u) fetch<G>(p, s, z, u0, v_next);
-        if (mirror) store_columns16<G>(o, bits(P + z * stride), ld, u0, v0, s.U, s.V, 16);
-        store_rows16<G>(o, bits(P + z * stride), ld, u0, v0, s.U, s.V, 16);
+        if (where == PART_BELOW) store_columns16<G>(o, bits(P + z * stride), ld, u0, v0, s.U, s.V, 16);
+        if (where != PART_ABOVE) store_rows16<G>(o, bits(P + z * stride), ld, u0, v0, s.U, s.V, 16);
     }
     __device__ void end(State&, unsigned, unsigned) const {}
 };
@@ -319,7 +318,7 @@ struct UpdateTerm {
 };
 
 struct EpiUpdate {
-    static constexpr bool kChained = true;
+    static constexpr bool kChained = true, kHeavy = true;
     struct State { float a, sum; };
     template <int G> using Pre = UpdateTerm::Pre<G>;
     UpdateTerm t;
@@ -332,7 +331,7 @@ struct EpiUpdate {
     }
     template <int G> __device__ void fetch(Pre<G>& p, const Shape& s, unsigned z, unsigned u0, unsigned v0) const { t.fetch<G>(p, s, z, u0, v0); }
     template <int G>
-    __device__ void chunk(State& st, Pre<G>& p, const Shape& s, unsigned z, unsigned u0, unsigned v0, unsigned v_next, bool, float (&x)[4][G][2]) const
+    __device__ void chunk(State& st, Pre<G>& p, const Shape& s, unsigned z, unsigned u0, unsigned v0, unsigned v_next, int, float (&x)[4][G][2]) const
     {
         t.add<G>(p, s, v0, st.a, 1.f, x);
         if (v_next != ~0u) fetch<G>(p, s, z, u0, v_next);
@@ -370,7 +369,7 @@ struct EpiUpdate {
 };
 
 struct EpiOut {                                            // O <- alpha X + beta O
-    static constexpr bool kChained = true;
+    static constexpr bool kChained = true, kHeavy = true;
     struct State { float a; };
     template <int G> struct Pre { UpdateTerm::Pre<G> x; Bits16<G> o; };
     UpdateTerm t;
@@ -388,7 +387,7 @@ struct EpiOut {                                            // O <- alpha X + bet
         else load_rows16<G>(p.o, O + z * stride_o, ldo, u0, v0, s.U, s.V, align);
     }
     template <int G>
-    __device__ void chunk(State& st, Pre<G>& p, const Shape& s, unsigned z, unsigned u0, unsigned v0, unsigned v_next, bool, float (&x)[4][G][2]) const
+    __device__ void chunk(State& st, Pre<G>& p, const Shape& s, unsigned z, unsigned u0, unsigned v0, unsigned v_next, int, float (&x)[4][G][2]) const
     {
         t.add<G>(p.x, s, v0, st.a, alpha / SX, x);
         uint16_t* o = O + z * stride_o;

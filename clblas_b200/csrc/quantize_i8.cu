@@ -128,10 +128,16 @@ __global__ void __launch_bounds__(256) quantize_across_kernel(const T* __restric
     const size_t l0 = lines * rank / ranks, n = lines * (rank + 1) / ranks - l0;
     const T* x = X + l0 * ldx + i;
     signed char* q = Q + l0 * ldq + i;
+    // This warp's lines: l0 + warp, + 8, ...; `mine` of them, the first `held` in registers.  Addresses are stepped and the counts are
+    // 32-bit: the kernel is bound by instructions as much as by memory (55 of them per access took 30 us where these take 13).
+    const int mine = in && n > (size_t)warp ? (int)((n - warp + 7) / 8) : 0, held = min(mine, KEEP);
+    const size_t step = 8 * ldx, qstep = 8 * ldq;
+    x += warp * ldx;
+    q += warp * ldq;
     W kept[KEEP];
 #pragma unroll
-    for (int k = 0; k < KEEP; k++)
-        if (in && (size_t)(8 * k + warp) < n) kept[k] = *reinterpret_cast<const W*>(x + (size_t)(8 * k + warp) * ldx);
+    for (int k = 0; k < KEEP; k++, x += step)
+        if (k < held) kept[k] = *reinterpret_cast<const W*>(x);
     unsigned top[V] = {};
     auto join = [&](const W& w) {
 #pragma unroll
@@ -139,11 +145,10 @@ __global__ void __launch_bounds__(256) quantize_across_kernel(const T* __restric
     };
 #pragma unroll
     for (int k = 0; k < KEEP; k++)
-        if (in && (size_t)(8 * k + warp) < n) join(kept[k]);
-    if (in) {
+        if (k < held) join(kept[k]);
+    const T* rest = x;                                     // past the KEEP-th line
 #pragma unroll 4
-        for (size_t l = 8 * KEEP + warp; l < n; l += 8) join(*reinterpret_cast<const W*>(x + l * ldx));
-    }
+    for (int k = KEEP; k < mine; k++, x += step) join(*reinterpret_cast<const W*>(x));
 #pragma unroll
     for (int j = 0; j < V; j++) tops[warp][j * 32 + lane] = top[j];
     __syncthreads();
@@ -171,23 +176,22 @@ __global__ void __launch_bounds__(256) quantize_across_kernel(const T* __restric
     }
     // A CTA's maxima stay where they are until every other CTA has read them.
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    auto write = [&](const W& w, size_t l) {
-        if constexpr (V == 1) {
-            put<T, 1>(q + l * ldq, w, s[0]);
-        } else {
-            uint32_t b[V];
+    uint32_t mask = 0;                                     // bytes of the positions that are not all zero
 #pragma unroll
-            for (int j = 0; j < V; j++) b[j] = s[j].inv == 0.f ? 0u : quant_bits(to_f(w.t[j]), s[j]);
-            *reinterpret_cast<uint32_t*>(q + l * ldq) = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
-        }
+    for (int j = 0; j < V; j++) mask |= s[j].inv == 0.f ? 0u : 0xffu << (8 * j);
+    auto write = [&](const W& w) {
+        uint32_t b[V];
+#pragma unroll
+        for (int j = 0; j < V; j++) b[j] = quant_bits(to_f(w.t[j]), s[j]);
+        if constexpr (V == 1) *reinterpret_cast<unsigned char*>(q) = (unsigned char)(b[0] & mask);
+        else *reinterpret_cast<uint32_t*>(q) = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410) & mask;
+        q += qstep;
     };
-    if (in) {
 #pragma unroll
-        for (int k = 0; k < KEEP; k++)
-            if ((size_t)(8 * k + warp) < n) write(kept[k], 8 * k + warp);
+    for (int k = 0; k < KEEP; k++)
+        if (k < held) write(kept[k]);
 #pragma unroll 4
-        for (size_t l = 8 * KEEP + warp; l < n; l += 8) write(*reinterpret_cast<const W*>(x + l * ldx), l);
-    }
+    for (int k = KEEP; k < mine; k++, rest += step) write(*reinterpret_cast<const W*>(rest));
     __syncwarp();
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
