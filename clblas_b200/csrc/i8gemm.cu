@@ -35,7 +35,7 @@ template <> __device__ __forceinline__ float2 unpack16<__nv_bfloat16>(uint32_t h
 // C[u, v] <- alpha su[u] sv[v] acc + beta C[u, v].
 template <typename T>
 struct EpiScaled {
-    static constexpr bool kChained = false, kHeavy = sizeof(T) == 4;
+    static constexpr bool kHeavy = sizeof(T) == 4;
     struct State { float factor[4]; };
     template <int G> struct Pre { Bits16<G> c; };
     const float* su;                // scales of the rows u and the columns v; nullptr: ones

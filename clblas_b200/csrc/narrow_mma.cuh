@@ -218,7 +218,6 @@ __host__ __device__ inline void tile_coords(const Shape& s, unsigned t, unsigned
 // ---------------------------------------------------------------------------------------------------------------------
 // Epilogue.  A warp finishes chunks of 32 rows x 8 G columns, held as fragments x[g][k][e]: row 8 g + lane / 4, column
 // 8 k + 2 (lane % 4) + e.  What a functor has:
-//   kChained      a link of a chain of products: its successor may start as soon as all its CTAs have
 //   kHeavy        reads as much as it writes (for choose_plan)
 //   begin()       per thread and tile
 //   Pre, fetch()  what a chunk needs besides the accumulators, requested one chunk ahead
@@ -250,8 +249,10 @@ __device__ __forceinline__ uint32_t block_transpose(uint32_t v)
 }
 
 // 16-bit matrices (as raw bits): a lane's share of a chunk, by rows (16 bytes per 8 rows) or by fragments.
-// `align`: bytes by which base and pitch are aligned, 16, 4 or 2.  Below 16, at the matrix's edge and for chunks narrower than 32 columns
-// fragments are accessed directly, 4 or 2 bytes a lane.
+// `align`: bytes by which base and pitch are aligned, 16, 4 or 2; PADDED: 16, and a line may be read and written up to the next
+// multiple of 8 elements.  Below 16, at the edge of a matrix that is not padded and for chunks narrower than 32 columns fragments are
+// accessed directly, 4 or 2 bytes a lane.
+constexpr int PADDED = 32;
 template <int G>
 struct Bits16 {
     uint32_t h[4][G];                                       // [g][k]: two values of row 8 g + lane / 4, columns 8 k + 2 (lane % 4)
@@ -262,8 +263,9 @@ __device__ __forceinline__ void load_rows16(Bits16<G>& f, const uint16_t* base, 
 {
     const int lane = threadIdx.x & 31, q = lane & 3;
     const unsigned u = u0 + lane / 4;
-    if (G == 4 && align == 16 && v0 + 32 <= V) {
+    if (G == 4 && (align == PADDED || (align == 16 && v0 + 32 <= V))) {
         const uint16_t* p = base + (size_t)u * ld + v0 + 8 * q;
+        if (v0 + 8 * q >= V) return;
 #pragma unroll
         for (int g = 0; g < 4; g++, p += 8 * ld)
             if (u + 8 * g < U) *reinterpret_cast<uint4*>(f.h[g]) = *reinterpret_cast<const uint4*>(p);
@@ -286,7 +288,7 @@ template <int G>
 __device__ __forceinline__ void rows_to_fragments(Bits16<G>& f, unsigned v0, unsigned V, int align)
 {
     if constexpr (G == 4) {
-        if (align == 16 && v0 + 32 <= V) {
+        if (align == PADDED || (align == 16 && v0 + 32 <= V)) {
 #pragma unroll
             for (int g = 0; g < 4; g++) quad_transpose(f.h[g]);
         }
@@ -298,12 +300,12 @@ __device__ __forceinline__ void store_rows16(Bits16<G>& f, uint16_t* base, size_
     const int lane = threadIdx.x & 31, q = lane & 3;
     const unsigned u = u0 + lane / 4;
     if constexpr (G == 4) {
-        if (align == 16 && v0 + 32 <= V) {
+        if (align == PADDED || (align == 16 && v0 + 32 <= V)) {
             uint16_t* p = base + (size_t)u * ld + v0 + 8 * q;
 #pragma unroll
             for (int g = 0; g < 4; g++, p += 8 * ld) {
                 quad_transpose(f.h[g]);
-                if (u + 8 * g < U) *reinterpret_cast<uint4*>(p) = make_uint4(f.h[g][0], f.h[g][1], f.h[g][2], f.h[g][3]);
+                if (u + 8 * g < U && v0 + 8 * q < V) *reinterpret_cast<uint4*>(p) = make_uint4(f.h[g][0], f.h[g][1], f.h[g][2], f.h[g][3]);
             }
             return;
         }
@@ -335,9 +337,9 @@ __device__ __forceinline__ void store_columns16(const Bits16<G>& f, uint16_t* ba
 #pragma unroll
         for (int g = 0; g < 4; g++) r[g] = block_transpose(f.h[g][k]);
         uint16_t* p = base + (size_t)(v + 8 * k) * ld + u0;
-        if (align == 16 && u0 + 32 <= U) {
+        if (align == PADDED || (align == 16 && u0 + 32 <= U)) {
             quad_transpose(r);
-            if (v + 8 * k < V) *reinterpret_cast<uint4*>(p + 8 * q) = make_uint4(r[0], r[1], r[2], r[3]);
+            if (v + 8 * k < V && u0 + 8 * q < U) *reinterpret_cast<uint4*>(p + 8 * q) = make_uint4(r[0], r[1], r[2], r[3]);
         } else if (v + 8 * k < V) {
 #pragma unroll
             for (int g = 0; g < 4; g++) {
@@ -487,7 +489,7 @@ narrow_persistent_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_
     if (CG == 2) cluster_sync();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    if (Epi::kChained) pdl_launch_dependents();
+    pdl_launch_dependents();
     pdl_wait();
 
     if (warp == 0) {
@@ -626,7 +628,7 @@ narrow_split_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_const
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    if (Epi::kChained) pdl_launch_dependents();
+    pdl_launch_dependents();
     pdl_wait();
 
     if (warp == 0) {
@@ -777,8 +779,9 @@ cudaError_t launch(Kernel kernel, unsigned grid, unsigned cluster, int smem, cud
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = cluster;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    // The kernel may start (barriers, tensor memory, descriptors) while the one before it on the stream drains, and waits for it
-    // in pdl_wait(); links of a chain let their successor do so from their own start on (kChained).
+    // The kernel may start (barriers, tensor memory, descriptors) while the one before it on the stream drains, and waits for it in
+    // pdl_wait(); it lets its own successor do so from its start on.  One 256 x 1024 orthogonalisation, 17 launches: 170 -> 113 us; 48 x
+    // 8192 x 8192 products in a row: 17.3 -> 16.1 us each.
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
@@ -832,7 +835,7 @@ cudaError_t run_split(const Operand& p, const Operand& q, Shape s, const Epi& ep
 //   a slab of k, 256 x 256               0.30 for a lone tile, 0.37 with all SMs at it, 0.36 to 0.45 in later rounds, when
 //                                        the epilogues (0.45: `heavy` ones, that read as much as they write) share L2 with the loads
 //   a slab of k, 256 x 128               0.30, later 0.37
-//   an epilogue                          128 x 128: 5.0, 4.6, 4.2 with 1, 2, 4 CTAs at it (heavy: 6.3, 5.6, 4.5); 256 x 256: 5.0 (7.7), 256 x 128: 5.0 (7.0)
+//   an epilogue                          128 x 128: 5.0, 4.6, 4.2 with 1, 2, 4 CTAs at it (heavy: 6.3, 5.6, 4.5); 256 x 256: 5.0 (8.5), 256 x 128: 5.0 (7.0)
 // A round of a persistent kernel takes the longer of its slabs and the epilogue before; clusters of 4 fill 128 SMs, clusters of 8 (never the
 // best here) fewer.
 struct Plan { unsigned pairs, split; };               // one of the two is 0
@@ -847,7 +850,7 @@ inline Plan choose_plan(unsigned U, unsigned V, unsigned K, unsigned batch, int 
     Plan best{};
     double least = 1e30;
     auto consider = [&](Plan plan, double us) { if (us < least) { least = us; best = plan; } };
-    const double pairs = std::floor(sms / 2), t256 = tiles(256, 256), t128 = tiles(128, 128), e256 = heavy ? 7.7 : 5.0, e128 = heavy ? 7.0 : 5.0;
+    const double pairs = std::floor(sms / 2), t256 = tiles(256, 256), t128 = tiles(128, 128), e256 = heavy ? 8.5 : 5.0, e128 = heavy ? 7.0 : 5.0;
     consider({256, 0}, 5 + nk * (0.30 + 0.07 * std::fmin(1.0, t256 / pairs)) + e256 + (std::ceil(t256 / pairs) - 1) * std::fmax(nk * (heavy ? 0.45 : 0.36), e256));
     consider({128, 0}, 5 + nk * 0.30 + 0.7 * e128 + (std::ceil(tiles(256, 128) / pairs) - 1) * std::fmax(nk * 0.37, e128));
     if (kind == KIND_I8)

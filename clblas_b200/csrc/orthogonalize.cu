@@ -47,22 +47,17 @@ __device__ __forceinline__ float2 unpack(uint32_t h) { return __half22float2(*re
 
 // ---- norm and split ---------------------------------------------------------------------------------------------------
 
-// Eight consecutive elements, at most n of them valid.  VEC: 16-byte loads (aligned lines, a whole piece).
+// Eight consecutive elements, n of them valid, as loaded.  VEC: 16-byte loads (aligned lines, a whole piece).
+template <typename T> struct alignas(16) Eight { T t[8]; };
 template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T* p, unsigned n, float (&x)[8])
+__device__ __forceinline__ void load8(const T* p, unsigned n, Eight<T>& x)
 {
     if (VEC && n == 8) {
-        constexpr int W = 16 / sizeof(T);
-        struct alignas(16) Word { T t[W]; };
 #pragma unroll
-        for (int i = 0; i < 8 / W; i++) {
-            const Word w = reinterpret_cast<const Word*>(p)[i];
-#pragma unroll
-            for (int j = 0; j < W; j++) x[i * W + j] = to_f(w.t[j]);
-        }
+        for (int i = 0; i < (int)sizeof(Eight<T>) / 16; i++) reinterpret_cast<uint4*>(x.t)[i] = reinterpret_cast<const uint4*>(p)[i];
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = i < (int)n ? to_f(p[i]) : 0.f;
+        for (int i = 0; i < 8; i++) x.t[i] = i < (int)n ? p[i] : T(0.f);
     }
 }
 
@@ -84,10 +79,11 @@ __global__ void __launch_bounds__(256) sum_squares_kernel(const T* __restrict__ 
     unsigned c = at % per_line;
     double sum = 0;
     while (l < lines) {
-        float x[4][8];
+        constexpr int AHEAD = 16 / sizeof(T);              // 128 bytes a thread in flight
+        Eight<T> raw[AHEAD];
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            load8<T, VEC>(g + l * ld + 8 * (size_t)c, l < lines ? min(8u, len - 8 * c) : 0, x[k]);
+        for (int k = 0; k < AHEAD; k++) {
+            load8<T, VEC>(g + l * ld + 8 * (size_t)c, l < lines ? min(8u, len - 8 * c) : 0, raw[k]);
             l += dl;
             c += dc;
             if (c >= per_line) { c -= per_line; l++; }
@@ -95,14 +91,15 @@ __global__ void __launch_bounds__(256) sum_squares_kernel(const T* __restrict__ 
         // Eight squares are added in FP32 (within 2^-21) and joined to the 64-bit sum, since a conversion for every element would take
         // longer than the loads; pieces whose squares could leave FP32's range are converted one by one.  NaN passes either way.
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
+        for (int k = 0; k < AHEAD; k++) {
             float top = 0.f, low = 0.f;
 #pragma unroll
-            for (int j = 0; j < 8; j++) { top = fmaxf(top, fabsf(x[k][j])); low = fmaf(x[k][j], x[k][j], low); }
+            for (int j = 0; j < 8; j++) { const float v = to_f(raw[k].t[j]); top = fmaxf(top, fabsf(v)); low = fmaf(v, v, low); }
             double more = low;
             if (top > 1e18f || (top < 1e-15f && top > 0.f)) {
                 more = 0;
-                for (int j = 0; j < 8; j++) more = fma((double)x[k][j], (double)x[k][j], more);
+#pragma unroll
+                for (int j = 0; j < 8; j++) { const double v = to_f(raw[k].t[j]); more = fma(v, v, more); }
             }
             sum += more;
         }
@@ -135,11 +132,11 @@ __global__ void __launch_bounds__(256) split_kernel(const T* __restrict__ G, siz
     const int piece = threadIdx.x % 8;
     const size_t i = i0 + 8 * piece;
     const unsigned n = i < len ? (unsigned)min((size_t)8, len - i) : 0;
-    float x[2][8];
+    Eight<T> raw[2];
 #pragma unroll
     for (int h = 0; h < 2; h++) {
         const size_t l = l0 + threadIdx.x / 8 + 32 * h;
-        load8<T, VEC>(g + l * ld + i, l < lines ? n : 0, x[h]);
+        load8<T, VEC>(g + l * ld + i, l < lines ? n : 0, raw[h]);
     }
     pdl_wait();
     if (threadIdx.x < 32) {
@@ -158,10 +155,11 @@ __global__ void __launch_bounds__(256) split_kernel(const T* __restrict__ G, siz
     }
     __syncthreads();
     const float f0 = factors[0], f1 = factors[1];
+    float x[2][8];
 #pragma unroll
     for (int h = 0; h < 2; h++)
 #pragma unroll
-        for (int j = 0; j < 8; j++) x[h][j] = x[h][j] * f0 * f1;
+        for (int j = 0; j < 8; j++) x[h][j] = to_f(raw[h].t[j]) * f0 * f1;
     size_t out_line[2], out_at;
     bool write[2];
     if (!FLIP) {
@@ -219,7 +217,7 @@ __device__ __forceinline__ uint16_t* bits(__half* p) { return reinterpret_cast<u
 __device__ __forceinline__ const uint16_t* bits(const __half* p) { return reinterpret_cast<const uint16_t*>(p); }
 
 struct EpiGram {                                           // A <- X X' - t I
-    static constexpr bool kChained = true, kHeavy = false;
+    static constexpr bool kHeavy = false;
     struct State { float t; };
     template <int G> struct Pre {};
     __half* A; size_t ld, stride;
@@ -243,14 +241,14 @@ struct EpiGram {                                           // A <- X X' - t I
                 if (d == 1) b -= st.t;
                 o.h[g][k] = pack(a, b);
             }
-        if (where == PART_BELOW) store_columns16<G>(o, bits(A + z * stride), ld, u0, v0, s.U, s.V, 16);
-        if (where != PART_ABOVE) store_rows16<G>(o, bits(A + z * stride), ld, u0, v0, s.U, s.V, 16);
+        if (where == PART_BELOW) store_columns16<G>(o, bits(A + z * stride), ld, u0, v0, s.U, s.V, PADDED);
+        if (where != PART_ABOVE) store_rows16<G>(o, bits(A + z * stride), ld, u0, v0, s.U, s.V, PADDED);
     }
     __device__ void end(State&, unsigned, unsigned) const {}
 };
 
 struct EpiSquare {                                         // P <- (b + 2 c t) A + c A^2
-    static constexpr bool kChained = true, kHeavy = false;
+    static constexpr bool kHeavy = false;
     struct State { float b; };
     template <int G> struct Pre { Bits16<G> a; };
     const __half* A; __half* P; size_t ld, stride;
@@ -260,12 +258,12 @@ struct EpiSquare {                                         // P <- (b + 2 c t) A
     template <int G>
     __device__ void fetch(Pre<G>& p, const Shape& s, unsigned z, unsigned u0, unsigned v0) const
     {
-        load_rows16<G>(p.a, bits(A + z * stride), ld, u0, v0, s.U, s.V, 16);
+        load_rows16<G>(p.a, bits(A + z * stride), ld, u0, v0, s.U, s.V, PADDED);
     }
     template <int G>
     __device__ void chunk(State& st, Pre<G>& p, const Shape& s, unsigned z, unsigned u0, unsigned v0, unsigned v_next, int where, float (&x)[4][G][2]) const
     {
-        rows_to_fragments<G>(p.a, v0, s.V, 16);
+        rows_to_fragments<G>(p.a, v0, s.V, PADDED);
         const float f = c / SA;
         Bits16<G> o;
 #pragma unroll
@@ -276,8 +274,8 @@ struct EpiSquare {                                         // P <- (b + 2 c t) A
                 o.h[g][k] = pack(fmaf(st.b, a.x, f * x[g][k][0]), fmaf(st.b, a.y, f * x[g][k][1]));
             }
         if (v_next != ~0u) fetch<G>(p, s, z, u0, v_next);
-        if (where == PART_BELOW) store_columns16<G>(o, bits(P + z * stride), ld, u0, v0, s.U, s.V, 16);
-        if (where != PART_ABOVE) store_rows16<G>(o, bits(P + z * stride), ld, u0, v0, s.U, s.V, 16);
+        if (where == PART_BELOW) store_columns16<G>(o, bits(P + z * stride), ld, u0, v0, s.U, s.V, PADDED);
+        if (where != PART_ABOVE) store_rows16<G>(o, bits(P + z * stride), ld, u0, v0, s.U, s.V, PADDED);
     }
     __device__ void end(State&, unsigned, unsigned) const {}
 };
@@ -291,8 +289,8 @@ struct UpdateTerm {
     template <int G>
     __device__ void fetch(Pre<G>& p, const Shape& s, unsigned z, unsigned u0, unsigned v0) const
     {
-        load_rows16<G>(p.h, bits(hi + z * stride), ld, u0, v0, s.U, s.V, 16);
-        load_rows16<G>(p.l, bits(lo + z * stride), ld, u0, v0, s.U, s.V, 16);
+        load_rows16<G>(p.h, bits(hi + z * stride), ld, u0, v0, s.U, s.V, PADDED);
+        load_rows16<G>(p.l, bits(lo + z * stride), ld, u0, v0, s.U, s.V, PADDED);
     }
     __device__ float coefficient(unsigned z) const
     {
@@ -303,8 +301,8 @@ struct UpdateTerm {
     template <int G>
     __device__ void add(Pre<G>& p, const Shape& s, unsigned v0, float coefficient, float scale, float (&x)[4][G][2]) const
     {
-        rows_to_fragments<G>(p.h, v0, s.V, 16);
-        rows_to_fragments<G>(p.l, v0, s.V, 16);
+        rows_to_fragments<G>(p.h, v0, s.V, PADDED);
+        rows_to_fragments<G>(p.l, v0, s.V, PADDED);
         const float f = scale * ((c == 0.f ? b : 1.f) / SA), w = scale * coefficient;
 #pragma unroll
         for (int g = 0; g < 4; g++)
@@ -318,7 +316,7 @@ struct UpdateTerm {
 };
 
 struct EpiUpdate {
-    static constexpr bool kChained = true, kHeavy = true;
+    static constexpr bool kHeavy = true;
     struct State { float a, sum; };
     template <int G> using Pre = UpdateTerm::Pre<G>;
     UpdateTerm t;
@@ -354,8 +352,8 @@ struct EpiUpdate {
                 sum += in && (whole || v + 1 < s.V) ? b * b : 0.f;
             }
         st.sum += sum;
-        store_rows16<G>(h, bits(hi + z * t.stride), t.ld, u0, v0, s.U, s.V, 16);
-        store_rows16<G>(l, bits(lo + z * t.stride), t.ld, u0, v0, s.U, s.V, 16);
+        store_rows16<G>(h, bits(hi + z * t.stride), t.ld, u0, v0, s.U, s.V, PADDED);
+        store_rows16<G>(l, bits(lo + z * t.stride), t.ld, u0, v0, s.U, s.V, PADDED);
     }
     __device__ void end(State& st, unsigned z, unsigned) const
     {
@@ -369,7 +367,7 @@ struct EpiUpdate {
 };
 
 struct EpiOut {                                            // O <- alpha X + beta O
-    static constexpr bool kChained = true, kHeavy = true;
+    static constexpr bool kHeavy = true;
     struct State { float a; };
     template <int G> struct Pre { UpdateTerm::Pre<G> x; Bits16<G> o; };
     UpdateTerm t;
