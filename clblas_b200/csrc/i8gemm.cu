@@ -142,38 +142,45 @@ __global__ void scale_lines_kernel(T* C, size_t lines, size_t len, size_t ld, fl
     }
 }
 
-// dst[r][k] (row pitch ldd, a multiple of 16) <- src[k][r] (pitch lds).  128 x 128 bytes per CTA: words of four r are read
-// along r, 4 x 4 bytes are exchanged in registers, words of four k go to shared memory (word w of row r at w ^ (r / 4), free of
-// bank conflicts both ways) and leave as 128-byte rows.
-template <bool WORDS>
-__global__ void __launch_bounds__(256) transpose_bytes_kernel(unsigned char* __restrict__ dst, size_t ldd, const unsigned char* __restrict__ src,
-                                                              size_t lds, size_t rows, size_t K)
+// An operand on its way to k-contiguous lines of pitch ldd (a multiple of 16, so whole 16-byte words of a line may be written).
+struct PackJob {
+    unsigned char* dst; size_t ldd;
+    const unsigned char* src; size_t lds;
+    size_t rows, K;
+    bool transpose;                 // src[k][r] instead of src[r][k]
+    bool words;                     // transpose: base and pitch allow 4-byte loads
+    unsigned tiles_r;               // transpose: tiles of 128 rows
+    unsigned blocks;
+};
+
+// dst[r][k] <- src[k][r].  128 x 128 bytes per CTA: words of four r are read along r, 4 x 4 bytes are exchanged in registers,
+// words of four k go to shared memory (word w of row r at w ^ (r / 4), free of bank conflicts both ways) and leave as 128-byte rows.
+__device__ __forceinline__ void transpose_tile(const PackJob& j, unsigned block, uint32_t* tile)
 {
-    __shared__ uint32_t tile[128 * 32];
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const size_t r0 = (size_t)blockIdx.x * 128, k0 = (size_t)blockIdx.y * 128;
-    const size_t r = r0 + 4 * lane;
+    const size_t r0 = (size_t)(block % j.tiles_r) * 128, k0 = (size_t)(block / j.tiles_r) * 128, r = r0 + 4 * lane;
+    uint32_t w[4][4];
+#pragma unroll
+    for (int g = 0; g < 4; g++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const size_t k = k0 + 4 * (warp * 4 + g) + i;
+            const unsigned char* p = j.src + k * j.lds + r;
+            w[g][i] = 0;
+            if (k >= j.K) continue;
+            if (j.words && r + 4 <= j.rows) {
+                w[g][i] = *reinterpret_cast<const uint32_t*>(p);
+            } else {
+#pragma unroll
+                for (int b = 0; b < 4; b++)
+                    if (r + b < j.rows) w[g][i] |= (uint32_t)p[b] << (8 * b);
+            }
+        }
 #pragma unroll
     for (int g = 0; g < 4; g++) {
         const int kw = warp * 4 + g;                       // word of four k
-        uint32_t w[4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const size_t k = k0 + 4 * kw + i;
-            const unsigned char* p = src + k * lds + r;
-            w[i] = 0;
-            if (k < K) {
-                if (WORDS && r + 4 <= rows) {
-                    w[i] = *reinterpret_cast<const uint32_t*>(p);
-                } else {
-#pragma unroll
-                    for (int b = 0; b < 4; b++)
-                        if (r + b < rows) w[i] |= (uint32_t)p[b] << (8 * b);
-                }
-            }
-        }
-        const uint32_t a = __byte_perm(w[0], w[1], 0x5140), b = __byte_perm(w[2], w[3], 0x5140);      // bytes 0, 1 of each pair
-        const uint32_t c = __byte_perm(w[0], w[1], 0x7362), d = __byte_perm(w[2], w[3], 0x7362);      // bytes 2, 3
+        const uint32_t a = __byte_perm(w[g][0], w[g][1], 0x5140), b = __byte_perm(w[g][2], w[g][3], 0x5140);      // bytes 0, 1 of each pair
+        const uint32_t c = __byte_perm(w[g][0], w[g][1], 0x7362), d = __byte_perm(w[g][2], w[g][3], 0x7362);      // bytes 2, 3
         const uint32_t o[4] = {__byte_perm(a, b, 0x5410), __byte_perm(a, b, 0x7632), __byte_perm(c, d, 0x5410), __byte_perm(c, d, 0x7632)};
 #pragma unroll
         for (int i = 0; i < 4; i++) tile[(4 * lane + i) * 32 + (kw ^ lane)] = o[i];
@@ -181,48 +188,57 @@ __global__ void __launch_bounds__(256) transpose_bytes_kernel(unsigned char* __r
     __syncthreads();
     for (int i = warp; i < 128; i += 8) {
         const size_t row = r0 + i, k = k0 + 4 * lane;
-        if (row < rows && k < K) *reinterpret_cast<uint32_t*>(dst + row * ldd + k) = tile[i * 32 + (lane ^ (i / 4))];      // ldd covers the last word
+        if (row < j.rows && k < j.K) *reinterpret_cast<uint32_t*>(j.dst + row * j.ldd + k) = tile[i * 32 + (lane ^ (i / 4))];
     }
 }
 
-// dst[r][k] <- src[r][k] for a source of any alignment.  A word of dst is cut out of the two aligned source words that hold it
-// when both lie inside the row, and collected byte by byte at its ends.
-__global__ void __launch_bounds__(256) copy_bytes_kernel(unsigned char* __restrict__ dst, size_t ldd, const unsigned char* __restrict__ src,
-                                                         size_t lds, size_t rows, size_t K)
+// dst[r][k] <- src[r][k] for a source of any alignment, 16 bytes of dst a thread.  They are cut out of the five aligned words that
+// hold them when all of those lie inside the row, and collected byte by byte at its ends.
+__device__ __forceinline__ void copy_piece(const PackJob& j, unsigned block)
 {
-    const size_t words = (K + 3) / 4, total = rows * words;
-    for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (size_t)gridDim.x * blockDim.x) {
-        const size_t row = i / words, w = i % words;
-        const unsigned char* line = src + row * lds;
-        const unsigned char* p = line + 4 * w;
-        const unsigned mis = (unsigned)(reinterpret_cast<uintptr_t>(p) & 3u);
-        const unsigned char* q = p - mis;
-        uint32_t v = 0;
-        if (q >= line && q + (mis ? 8 : 4) <= line + K) {
-            const uint32_t lo = *reinterpret_cast<const uint32_t*>(q);
-            v = mis ? __funnelshift_r(lo, *reinterpret_cast<const uint32_t*>(q + 4), 8 * mis) : lo;
-        } else {
+    const unsigned per_row = (unsigned)((j.K + 15) / 16);
+    const size_t i = (size_t)block * 256 + threadIdx.x, row = i / per_row;
+    const unsigned k = (unsigned)(i - row * per_row) * 16;
+    if (row >= j.rows) return;
+    const unsigned char* line = j.src + row * j.lds;
+    const unsigned char* p = line + k;
+    const unsigned mis = (unsigned)(reinterpret_cast<uintptr_t>(p) & 3u);
+    const unsigned char* q = p - mis;
+    uint32_t o[4] = {};
+    if (q >= line && q + (mis ? 20 : 16) <= line + j.K) {
+        uint32_t w[5];
 #pragma unroll
-            for (int b = 0; b < 4; b++)
-                if (4 * w + b < K) v |= (uint32_t)p[b] << (8 * b);
-        }
-        *reinterpret_cast<uint32_t*>(dst + row * ldd + 4 * w) = v;
+        for (int b = 0; b < 4; b++) w[b] = reinterpret_cast<const uint32_t*>(q)[b];
+        w[4] = mis ? reinterpret_cast<const uint32_t*>(q)[4] : 0;
+#pragma unroll
+        for (int b = 0; b < 4; b++) o[b] = __funnelshift_r(w[b], w[b + 1], 8 * mis);
+    } else {
+#pragma unroll
+        for (int b = 0; b < 16; b++)
+            if (k + b < j.K) o[b / 4] |= (uint32_t)p[b] << (8 * (b % 4));
     }
+    *reinterpret_cast<uint4*>(j.dst + row * j.ldd + k) = make_uint4(o[0], o[1], o[2], o[3]);
 }
 
-cudaError_t pack_operand(unsigned char* dst, size_t ldd, const void* src, size_t lds, size_t rows, size_t K, bool transpose, cudaStream_t s)
+// Both operands of a product in one launch (either may have no blocks).
+__global__ void __launch_bounds__(256) pack_kernel(const PackJob a, const PackJob b)
 {
-    const unsigned char* p = static_cast<const unsigned char*>(src);
-    if (transpose) {
-        const dim3 grid((unsigned)((rows + 127) / 128), (unsigned)((K + 127) / 128));
-        if (((reinterpret_cast<uintptr_t>(p) | lds) & 3u) == 0) transpose_bytes_kernel<true><<<grid, 256, 0, s>>>(dst, ldd, p, lds, rows, K);
-        else transpose_bytes_kernel<false><<<grid, 256, 0, s>>>(dst, ldd, p, lds, rows, K);
-    } else {
-        const size_t total = rows * ((K + 3) / 4), want = (total + 255) / 256, most = (size_t)sm_count() * 16;
-        copy_bytes_kernel<<<(unsigned)(want < most ? want : most), 256, 0, s>>>(dst, ldd, p, lds, rows, K);
-    }
-    count_launch();
-    return cudaGetLastError();
+    __shared__ uint32_t tile[128 * 32];
+    pdl_launch_dependents();
+    pdl_wait();
+    const bool first = blockIdx.x < a.blocks;
+    const PackJob& j = first ? a : b;
+    const unsigned block = first ? blockIdx.x : blockIdx.x - a.blocks;
+    if (j.transpose) transpose_tile(j, block, tile);
+    else copy_piece(j, block);
+}
+
+PackJob pack_job(unsigned char* dst, size_t ldd, const signed char* src, size_t lds, size_t rows, size_t K, bool transpose)
+{
+    PackJob j{dst, ldd, reinterpret_cast<const unsigned char*>(src), lds, rows, K, transpose, ((reinterpret_cast<uintptr_t>(src) | lds) & 3u) == 0, (unsigned)((rows + 127) / 128), 0};
+    const size_t blocks = transpose ? j.tiles_r * ((K + 127) / 128) : (rows * ((K + 15) / 16) + 255) / 256;
+    j.blocks = blocks < (1u << 30) ? (unsigned)blocks : 0;
+    return j;
 }
 
 template <typename T>
@@ -283,14 +299,18 @@ cudaError_t i8gemm_typed(const I8GemmProblem& p, cudaStream_t s)
     if (fixP || fixQ) {
         const size_t pn = fixP ? kld * p.lines : 0, qn = fixQ ? kld * p.len : 0, at = (pn + 255) / 256 * 256;
         if ((e = ws_alloc(reinterpret_cast<void**>(&ws), at + qn, s)) != cudaSuccess) return e;
+        PackJob jobs[2] = {};
         if (fixP) {
-            e = pack_operand(ws, kld, p.P, p.ldp, p.lines, p.K, !p.p_kcontig, s);
+            jobs[0] = pack_job(ws, kld, p.P, p.ldp, p.lines, p.K, !p.p_kcontig);
             a.base = ws; a.ld = kld;
         }
-        if (e == cudaSuccess && fixQ) {
-            e = pack_operand(ws + at, kld, p.Q, p.ldq, p.len, p.K, !p.q_kcontig, s);
+        if (fixQ) {
+            jobs[1] = pack_job(ws + at, kld, p.Q, p.ldq, p.len, p.K, !p.q_kcontig);
             b.base = ws + at; b.ld = kld;
         }
+        if ((fixP && jobs[0].blocks == 0) || (fixQ && jobs[1].blocks == 0)) e = cudaErrorNotSupported;
+        else e = launch_chained(pack_kernel, dim3(jobs[0].blocks + jobs[1].blocks), 256, s, jobs[0], jobs[1]);
+        if (e == cudaSuccess) count_launch();
     }
     if (e == cudaSuccess) e = multiply<T>(a, b, p.s_lines, p.s_len, p.alpha, p.beta, C, p.ldc, s);
     if (ws) {

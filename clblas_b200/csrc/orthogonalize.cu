@@ -418,22 +418,6 @@ struct EpiOut {                                            // O <- alpha X + bet
 
 // ---- the chain ----------------------------------------------------------------------------------------------------------
 
-// A plain kernel as a link of the chain: it may start while the one before it drains and waits in pdl_wait().
-template <typename... KArgs, typename... Args>
-cudaError_t launch_chained(void (*kernel)(KArgs...), dim3 grid, unsigned block, cudaStream_t s, Args... args)
-{
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(block);
-    cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
-
 template <typename T>
 cudaError_t orthogonalize_typed(const OrthProblem& p, cudaStream_t s)
 {
