@@ -251,6 +251,14 @@ void ws_release_all();
 // through ws_alloc, so a call during which this does not move allocated nothing).
 unsigned long long ws_alloc_count();
 
+// Set-up steps that are no stream work (creating a pool, a kernel's attributes) may fall into a call that is being captured; in
+// the relaxed mode they neither fail nor spoil the capture.  Holds for the calling thread while it lives.
+struct RelaxedCapture {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+    ~RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+};
+
 // One-time, per-device set-up step (a kernel's opt-in to large dynamic shared memory) that several host
 // threads may reach at once: the step is idempotent, the flag is atomic.
 struct DeviceOnce {
@@ -262,6 +270,7 @@ struct DeviceOnce {
         cudaGetDevice(&dev);
         const bool tracked = dev >= 0 && dev < 64;
         if (tracked && done[dev].load(std::memory_order_acquire)) return cudaSuccess;
+        RelaxedCapture relaxed;
         const cudaError_t e = step();
         if (e != cudaSuccess) return e;
         if (tracked) done[dev].store(1, std::memory_order_release);

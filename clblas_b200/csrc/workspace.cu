@@ -24,6 +24,7 @@ cudaError_t pool_for_current_device(cudaMemPool_t* out)
     if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
     std::lock_guard<std::mutex> lock(g_mu);
     if (g_pool[dev] == nullptr) {
+        RelaxedCapture relaxed;
         cudaMemPoolProps props = {};
         props.allocType = cudaMemAllocationTypePinned;
         props.handleTypes = cudaMemHandleTypeNone;
