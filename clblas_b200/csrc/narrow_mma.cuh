@@ -766,22 +766,6 @@ inline void set_tiles(Shape& s, unsigned bu, unsigned bv)
     s.tiles = s.tri ? s.per * (s.tilesU * (s.tilesU + 1) / 2) : s.tilesU * s.tilesV;
 }
 
-// A plain kernel that waits for the one before it on the stream in pdl_wait().
-template <typename... KArgs, typename... Args>
-cudaError_t launch_chained(void (*kernel)(KArgs...), dim3 grid, unsigned block, cudaStream_t s, Args... args)
-{
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(block);
-    cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
-
 template <typename Kernel, typename Epi>
 cudaError_t launch(Kernel kernel, unsigned grid, unsigned cluster, int smem, cudaStream_t st, const CUtensorMap& mp, const CUtensorMap& mq,
                    const Shape& s, const Epi& epi)

@@ -6,6 +6,7 @@
 //
 // Bound by memory: each element is read once and one byte written.
 #include "common.h"
+#include "tma_pipeline.cuh"
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -77,6 +78,8 @@ __global__ void __launch_bounds__(THREADS) quantize_lines_kernel(const T* __rest
     const T* x = X + (size_t)blockIdx.x * ldx;
     signed char* q = Q + (size_t)blockIdx.x * ldq;
     const size_t pieces = len / V;
+    pdl_launch_dependents();
+    pdl_wait();
     W kept[KEEP];
     unsigned top = 0;
 #pragma unroll
@@ -128,6 +131,8 @@ __global__ void __launch_bounds__(256) quantize_across_kernel(const T* __restric
     const size_t l0 = lines * rank / ranks, n = lines * (rank + 1) / ranks - l0;
     const T* x = X + l0 * ldx + i;
     signed char* q = Q + l0 * ldq + i;
+    pdl_launch_dependents();
+    pdl_wait();
     // This warp's lines: l0 + warp, + 8, ...; `mine` of them, the first `held` in registers.  Addresses are stepped and the counts are
     // 32-bit: the kernel is bound by instructions as much as by memory (55 of them per access took 30 us where these take 13).
     const int mine = in && n > (size_t)warp ? (int)((n - warp + 7) / 8) : 0, held = min(mine, KEEP);
@@ -208,12 +213,14 @@ cudaError_t launch_across(const T* X, size_t ldx, signed char* Q, size_t ldq, fl
     cfg.gridDim = dim3((unsigned)(strips * ranks));
     cfg.blockDim = dim3(256);
     cfg.stream = s;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = ranks;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = 2;
     count_launch();
     return cudaLaunchKernelEx(&cfg, quantize_across_kernel<T, V, KEEP>, X, ldx, Q, ldq, scale, lines, len);
 }
@@ -228,16 +235,15 @@ cudaError_t quantize_typed(bool per_line, const T* X, size_t ldx, signed char* Q
         return launch_across<T, 1, 64>(X, ldx, Q, ldq, scale, lines, len, s);
     }
     if (lines >= (1u << 31)) return cudaErrorNotSupported;
+    count_launch();
     const unsigned grid = (unsigned)lines;
     // 64 elements a thread in registers.  8192 x 8192 BF16: 33 us with 128 threads a line (6.1 TB/s, 94 % of a copy's rate), 36 with 64 or
     // 256 of 32 elements each, 42 with 512; so as few threads as hold the line.
     if (aligned16(X) && (ldx * sizeof(T)) % 16 == 0 && (reinterpret_cast<uintptr_t>(Q) | ldq) % V == 0) {
-        if (len <= 128 * 64) quantize_lines_kernel<T, 128, V, 64 / V><<<grid, 128, 0, s>>>(X, ldx, Q, ldq, scale, len);
-        else                 quantize_lines_kernel<T, 256, V, 64 / V><<<grid, 256, 0, s>>>(X, ldx, Q, ldq, scale, len);
-    } else
-        quantize_lines_kernel<T, 256, 1, 32><<<grid, 256, 0, s>>>(X, ldx, Q, ldq, scale, len);
-    count_launch();
-    return cudaGetLastError();
+        if (len <= 128 * 64) return launch_chained(quantize_lines_kernel<T, 128, V, 64 / V>, dim3(grid), 128, s, X, ldx, Q, ldq, scale, len);
+        return launch_chained(quantize_lines_kernel<T, 256, V, 64 / V>, dim3(grid), 256, s, X, ldx, Q, ldq, scale, len);
+    }
+    return launch_chained(quantize_lines_kernel<T, 256, 1, 32>, dim3(grid), 256, s, X, ldx, Q, ldq, scale, len);
 }
 
 }  // namespace
