@@ -20,7 +20,7 @@
 //   * Accumulators and everything between accumulator and store are FP32.  X is held times 2^12, A and P times 2^8, so that the
 //     entries of large matrices (about 1/sqrt(m)) stay far above FP16's smallest numbers.
 // The result is good to about 1e-3 and is therefore given in BF16 only.
-#include "narrow_mma.cuh"
+#include "orthogonalize.cuh"
 
 #include <algorithm>
 #include <type_traits>
@@ -30,20 +30,6 @@ namespace cb200 {
 namespace {
 
 using namespace narrow;
-
-constexpr float SX = 4096.f, SA = 256.f;                  // scales of the stored X and of the stored A, P
-constexpr double SUM_UNIT = 16777216.0;                    // sums of squares are counted in 2^-24
-constexpr double EPS = 1e-7;
-
-typedef unsigned long long u64;
-
-template <typename T> __device__ __forceinline__ float to_f(T v);
-template <> __device__ __forceinline__ float to_f(float v) { return v; }
-template <> __device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
-template <> __device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
-
-__device__ __forceinline__ uint32_t pack(float a, float b) { const __half2 h = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t*>(&h); }
-__device__ __forceinline__ float2 unpack(uint32_t h) { return __half22float2(*reinterpret_cast<const __half2*>(&h)); }
 
 // ---- norm and split ---------------------------------------------------------------------------------------------------
 
@@ -88,20 +74,12 @@ __global__ void __launch_bounds__(256) sum_squares_kernel(const T* __restrict__ 
             c += dc;
             if (c >= per_line) { c -= per_line; l++; }
         }
-        // Eight squares are added in FP32 (within 2^-21) and joined to the 64-bit sum, since a conversion for every element would take
-        // longer than the loads; pieces whose squares could leave FP32's range are converted one by one.  NaN passes either way.
 #pragma unroll
         for (int k = 0; k < AHEAD; k++) {
-            float top = 0.f, low = 0.f;
+            float v[8];
 #pragma unroll
-            for (int j = 0; j < 8; j++) { const float v = to_f(raw[k].t[j]); top = fmaxf(top, fabsf(v)); low = fmaf(v, v, low); }
-            double more = low;
-            if (top > 1e18f || (top < 1e-15f && top > 0.f)) {
-                more = 0;
-#pragma unroll
-                for (int j = 0; j < 8; j++) { const double v = to_f(raw[k].t[j]); more = fma(v, v, more); }
-            }
-            sum += more;
+            for (int j = 0; j < 8; j++) v[j] = to_f(raw[k].t[j]);
+            sum += sum_of_squares(v);
         }
     }
     double all = sum;
@@ -144,13 +122,9 @@ __global__ void __launch_bounds__(256) split_kernel(const T* __restrict__ G, siz
         for (int k = threadIdx.x; k < parts; k += 32) sum += part[(size_t)z * parts + k];
         for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
         if (threadIdx.x == 0) {
-            // The factor SX / (norm + eps) may lie outside FP32: a power of two and a number in [1, 2).
-            const double norm = sqrt(sum), f = 1.0 / (norm + EPS);
-            int e;
-            const double m = frexp(f * SX, &e);
-            factors[0] = isfinite(norm) ? (float)ldexp(1.0, e - 1) : nanf("");
-            factors[1] = (float)(2.0 * m);
-            if (blockIdx.x == 0) sums[(size_t)z * sums_pitch] = isfinite(norm) ? (u64)(norm * f * norm * f * SUM_UNIT) : 0;
+            double square;
+            norm_factors(sqrt(sum), factors[0], factors[1], square);
+            if (blockIdx.x == 0) sums[(size_t)z * sums_pitch] = (u64)(square * SUM_UNIT);
         }
     }
     __syncthreads();
@@ -203,13 +177,10 @@ __global__ void __launch_bounds__(256) split_kernel(const T* __restrict__ G, siz
 
 // ---- epilogues ----------------------------------------------------------------------------------------------------------
 
-// The shift t: the mean diagonal of X X', once most singular values have come near one; 0 before (and for a matrix of NaN, whose
-// sum says nothing).  While X is dominated by a few directions the shift would put roundings of t on all the others
-// (rank 8 of 100: 3e-3 with t from the first step on, 7e-4 from t = 0.2 on).
+// The shift from the gathered sum of squares.
 __device__ __forceinline__ float shift_of(const u64* sums, size_t at, float inv_n)
 {
-    const float t = (float)((double)__ldcg(sums + at) * (1.0 / SUM_UNIT)) * inv_n;       // past L1: a neighbour is added to meanwhile
-    return t >= 0.2f ? t : 0.f;
+    return shift((float)((double)__ldcg(sums + at) * (1.0 / SUM_UNIT)) * inv_n);       // past L1: a neighbour is added to meanwhile
 }
 
 // The workspaces have a pitch of a multiple of 8 elements: every row piece is aligned.
@@ -421,6 +392,7 @@ struct EpiOut {                                            // O <- alpha X + bet
 template <typename T>
 cudaError_t orthogonalize_typed(const OrthProblem& p, cudaStream_t s)
 {
+    if (orthogonalize_small_applies(p)) return orthogonalize_small<T>(p, s);
     const bool flip = p.lines > p.len;
     const size_t n = flip ? p.len : p.lines, m = flip ? p.lines : p.len, batch = p.batch;
     if (m >= (1u << 31) || batch >= 65536) return cudaErrorNotSupported;
@@ -497,6 +469,6 @@ cudaError_t orthogonalize(const OrthProblem& p, cudaStream_t s)
     }
 }
 
-unsigned orthogonalize_fault_flag() { return read_wait_timeout_flag(); }
+unsigned orthogonalize_fault_flag() { return read_wait_timeout_flag() | orthogonalize_small_fault_flag(); }
 
 }  // namespace cb200
