@@ -8,6 +8,8 @@
 #include "common.h"
 #include "tma_pipeline.cuh"
 
+#include <algorithm>
+
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -112,102 +114,180 @@ __global__ void __launch_bounds__(THREADS) quantize_lines_kernel(const T* __rest
         }
 }
 
-// One scale per position of the lines: the maximum runs across the lines.  A cluster takes a strip of 32 V positions; its CTAs share the
-// lines, a warp a line at a time.  Each thread keeps its first KEEP accesses in registers, the maxima meet in distributed shared
-// memory, and every CTA quantises its own lines: one launch, each element read once (lines beyond 8 KEEP per CTA twice, the second
-// time from L2).  Two passes over the matrix with atomic maxima in between took 31 us for 4099 x 2300 FP32 with their memset.
-template <typename T, int V, int KEEP>
+// One scale per position of the lines: the maximum runs across the lines.
+//
+// Up to 5120 lines, unless the matrix is large and aligned: a cluster takes a strip of 32 positions, its CTAs share the lines, a warp a line at a time.  Each
+// thread keeps its elements in registers, the maxima meet in distributed shared memory and every CTA quantises its own lines:
+// one launch, each element read once.  KEEP elements a thread: 64, or the 80 that two CTAs per SM have room for when that saves a pass.
+template <typename T, int KEEP>
 __global__ void __launch_bounds__(256) quantize_across_kernel(const T* __restrict__ X, size_t ldx, signed char* __restrict__ Q, size_t ldq,
                                                               float* __restrict__ scale, size_t lines, size_t len)
 {
-    typedef Word<T, V> W;
-    __shared__ unsigned tops[8][32 * V], joined[32 * V];
+    __shared__ unsigned tops[8][32], joined[32];
     uint32_t rank, ranks;
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const size_t i = ((size_t)(blockIdx.x / ranks) * 32 + lane) * V;
-    const bool in = i < len;                               // V > 1 only where V divides len
+    const size_t i = (size_t)(blockIdx.x / ranks) * 32 + lane;
+    const bool in = i < len;
     const size_t l0 = lines * rank / ranks, n = lines * (rank + 1) / ranks - l0;
-    const T* x = X + l0 * ldx + i;
-    signed char* q = Q + l0 * ldq + i;
     pdl_launch_dependents();
     pdl_wait();
-    // This warp's lines: l0 + warp, + 8, ...; `mine` of them, the first `held` in registers.  Addresses are stepped and the counts are
-    // 32-bit: the kernel is bound by instructions as much as by memory (55 of them per access took 30 us where these take 13).
-    const int mine = in && n > (size_t)warp ? (int)((n - warp + 7) / 8) : 0, held = min(mine, KEEP);
+    // This lane's lines: l0 + warp, + 8, ...  Addresses are stepped and the count is 32-bit: the kernel is bound by instructions as
+    // much as by memory (55 of them per access took 30 us where 22 took 20).
+    const int mine = in && n > (size_t)warp ? (int)((n - warp + 7) / 8) : 0;        // at most KEEP
     const size_t step = 8 * ldx, qstep = 8 * ldq;
-    x += warp * ldx;
-    q += warp * ldq;
-    W kept[KEEP];
+    const T* x = X + (l0 + warp) * ldx + i;
+    signed char* q = Q + (l0 + warp) * ldq + i;
+    T kept[KEEP];
 #pragma unroll
     for (int k = 0; k < KEEP; k++, x += step)
-        if (k < held) kept[k] = *reinterpret_cast<const W*>(x);
-    unsigned top[V] = {};
-    auto join = [&](const W& w) {
-#pragma unroll
-        for (int j = 0; j < V; j++) top[j] = max(top[j], magnitude(to_f(w.t[j])));
-    };
+        if (k < mine) kept[k] = *x;
+    unsigned top = 0;
 #pragma unroll
     for (int k = 0; k < KEEP; k++)
-        if (k < held) join(kept[k]);
-    const T* rest = x;                                     // past the KEEP-th line
-#pragma unroll 4
-    for (int k = KEEP; k < mine; k++, x += step) join(*reinterpret_cast<const W*>(x));
-#pragma unroll
-    for (int j = 0; j < V; j++) tops[warp][j * 32 + lane] = top[j];
+        if (k < mine) top = max(top, magnitude(to_f(kept[k])));
+    tops[warp][lane] = top;
     __syncthreads();
-    for (int j = threadIdx.x; j < 32 * V; j += 256) {
-        unsigned m = tops[0][j];
+    if (warp == 0) {
 #pragma unroll
-        for (int w = 1; w < 8; w++) m = max(m, tops[w][j]);
-        joined[j] = m;
+        for (int w = 1; w < 8; w++) top = max(top, tops[w][lane]);
+        joined[lane] = top;
     }
+    __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-    LineScale s[V];
-#pragma unroll
-    for (int j = 0; j < V; j++) {
-        unsigned m = 0;
-        const uint32_t here = static_cast<uint32_t>(__cvta_generic_to_shared(&joined[j * 32 + lane]));
-        for (uint32_t r = 0; r < ranks; r++) {
-            uint32_t there, v;
-            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(here), "r"(r));
-            asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(there) : "memory");
-            m = max(m, v);
-        }
-        s[j] = line_scale(m);
-        if (rank == 0 && warp == 0 && in) scale[i + j] = s[j].s;
+    unsigned m = 0;
+    const uint32_t here = static_cast<uint32_t>(__cvta_generic_to_shared(&joined[lane]));
+    for (uint32_t r = 0; r < ranks; r++) {
+        uint32_t there, v;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(here), "r"(r));
+        asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(there) : "memory");
+        m = max(m, v);
     }
+    const LineScale s = line_scale(m);
+    if (rank == 0 && warp == 0 && in) scale[i] = s.s;
     // A CTA's maxima stay where they are until every other CTA has read them.
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    uint32_t mask = 0;                                     // bytes of the positions that are not all zero
+    const uint32_t mask = s.inv == 0.f ? 0u : 0xffu;
 #pragma unroll
-    for (int j = 0; j < V; j++) mask |= s[j].inv == 0.f ? 0u : 0xffu << (8 * j);
-    auto write = [&](const W& w) {
-        uint32_t b[V];
-#pragma unroll
-        for (int j = 0; j < V; j++) b[j] = quant_bits(to_f(w.t[j]), s[j]);
-        if constexpr (V == 1) *reinterpret_cast<unsigned char*>(q) = (unsigned char)(b[0] & mask);
-        else *reinterpret_cast<uint32_t*>(q) = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410) & mask;
-        q += qstep;
-    };
-#pragma unroll
-    for (int k = 0; k < KEEP; k++)
-        if (k < held) write(kept[k]);
-#pragma unroll 4
-    for (int k = KEEP; k < mine; k++, rest += step) write(*reinterpret_cast<const W*>(rest));
+    for (int k = 0; k < KEEP; k++, q += qstep)
+        if (k < mine) *q = (signed char)(quant_bits(to_f(kept[k]), s) & mask);
     __syncwarp();
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-template <typename T, int V, int KEEP>
-cudaError_t launch_across(const T* X, size_t ldx, signed char* Q, size_t ldq, float* scale, size_t lines, size_t len, cudaStream_t s)
+// Everything larger: two passes, the second one mostly from L2.  A CTA takes COLS V positions and a block of lines, a warp 32 / COLS
+// lines at a time, AHEAD accesses in flight.  First the maxima of every block, then the maximum over the blocks and the quantisation.
+template <typename T, int V, int COLS>
+struct AcrossBlock {
+    typedef Word<T, V> W;
+    static constexpr int RPW = 32 / COLS, AHEAD = V == 1 ? 16 : 8;
+    size_t i, l0;
+    int mine;                                                  // this lane's lines: l0, + 8 RPW, ...
+    __device__ AcrossBlock(size_t lines, size_t len, unsigned blocks)
+    {
+        const int lane = threadIdx.x % 32, line = (int)(threadIdx.x / 32) * RPW + lane / COLS;
+        i = ((size_t)blockIdx.x * COLS + lane % COLS) * V;
+        const size_t first = lines * blockIdx.y / blocks, n = lines * (blockIdx.y + 1) / blocks - first;
+        l0 = first + line;
+        mine = i < len && n > (size_t)line ? (int)((n - line + 8 * RPW - 1) / (8 * RPW)) : 0;
+    }
+};
+
+template <typename T, int V, int COLS>
+__global__ void __launch_bounds__(256) across_max_kernel(const T* __restrict__ X, size_t ldx, unsigned* __restrict__ tops, size_t lines, size_t len)
 {
-    const size_t strips = (len + 32 * V - 1) / (32 * V);
-    // CTAs per strip: no more than keep all lines in registers, and enough of them to fill the machine twice over.
-    unsigned ranks = 1;
-    while (ranks < 8 && lines > (size_t)8 * ranks && (lines > (size_t)8 * KEEP * ranks || strips * ranks < 2 * (size_t)sm_count())) ranks *= 2;
+    typedef AcrossBlock<T, V, COLS> B;
+    __shared__ unsigned per_warp[8][COLS * V];
+    pdl_launch_dependents();
+    pdl_wait();
+    const B b(lines, len, gridDim.y);
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const T* x = X + b.l0 * ldx + b.i;
+    const size_t step = 8 * B::RPW * ldx;
+    unsigned top[V] = {};
+    for (int k = 0; k < b.mine; k += B::AHEAD) {
+        typename B::W v[B::AHEAD];
+#pragma unroll
+        for (int j = 0; j < B::AHEAD; j++, x += step)
+            if (k + j < b.mine) v[j] = *reinterpret_cast<const typename B::W*>(x);
+#pragma unroll
+        for (int j = 0; j < B::AHEAD; j++)
+            if (k + j < b.mine) {
+#pragma unroll
+                for (int e = 0; e < V; e++) top[e] = max(top[e], magnitude(to_f(v[j].t[e])));
+            }
+    }
+#pragma unroll
+    for (int e = 0; e < V; e++) {
+#pragma unroll
+        for (int d = 16; d >= COLS; d >>= 1) top[e] = max(top[e], __shfl_xor_sync(0xffffffffu, top[e], d));
+        if (lane < COLS) per_warp[warp][lane * V + e] = top[e];
+    }
+    __syncthreads();
+    for (int j = threadIdx.x; j < COLS * V; j += 256) {
+        const size_t at = (size_t)blockIdx.x * COLS * V + j;
+        unsigned m = per_warp[0][j];
+#pragma unroll
+        for (int w = 1; w < 8; w++) m = max(m, per_warp[w][j]);
+        if (at < len) tops[(size_t)blockIdx.y * len + at] = m;
+    }
+}
+
+template <typename T, int V, int COLS>
+__global__ void __launch_bounds__(256) across_quantize_kernel(const T* __restrict__ X, size_t ldx, signed char* __restrict__ Q, size_t ldq,
+                                                              const unsigned* __restrict__ tops, float* __restrict__ scale, size_t lines, size_t len)
+{
+    typedef AcrossBlock<T, V, COLS> B;
+    __shared__ unsigned joined[COLS * V];
+    pdl_launch_dependents();
+    pdl_wait();
+    const B b(lines, len, gridDim.y);
+    for (int j = threadIdx.x; j < COLS * V; j += 256) {
+        const size_t at = (size_t)blockIdx.x * COLS * V + j;
+        unsigned m = 0;
+        if (at < len) {
+#pragma unroll 8
+            for (unsigned y = 0; y < gridDim.y; y++) m = max(m, __ldcg(tops + (size_t)y * len + at));
+            if (blockIdx.y == 0) scale[at] = line_scale(m).s;
+        }
+        joined[j] = m;
+    }
+    __syncthreads();
+    LineScale s[V];
+    uint32_t mask[(V + 3) / 4] = {};                           // bytes of the positions that are not all zero
+#pragma unroll
+    for (int e = 0; e < V; e++) {
+        s[e] = line_scale(joined[(threadIdx.x % COLS) * V + e]);
+        mask[e / 4] |= s[e].inv == 0.f ? 0u : 0xffu << (8 * (e % 4));
+    }
+    const T* x = X + b.l0 * ldx + b.i;
+    signed char* q = Q + b.l0 * ldq + b.i;
+    const size_t step = 8 * B::RPW * ldx, qstep = 8 * B::RPW * ldq;
+    for (int k = 0; k < b.mine; k += B::AHEAD) {
+        typename B::W v[B::AHEAD];
+#pragma unroll
+        for (int j = 0; j < B::AHEAD; j++, x += step)
+            if (k + j < b.mine) v[j] = *reinterpret_cast<const typename B::W*>(x);
+#pragma unroll
+        for (int j = 0; j < B::AHEAD; j++, q += qstep) {
+            if (k + j >= b.mine) continue;
+            uint32_t r[V];
+#pragma unroll
+            for (int e = 0; e < V; e++) r[e] = quant_bits(to_f(v[j].t[e]), s[e]);
+            auto four = [&](int e) { return __byte_perm(__byte_perm(r[e], r[e + 1], 0x0040), __byte_perm(r[e + 2], r[e + 3], 0x0040), 0x5410) & mask[e / 4]; };
+            if constexpr (V == 1) *q = (signed char)(r[0] & mask[0]);
+            else if constexpr (V == 4) *reinterpret_cast<uint32_t*>(q) = four(0);
+            else *reinterpret_cast<uint2*>(q) = make_uint2(four(0), four(4));
+        }
+    }
+}
+
+template <typename T, int KEEP>
+cudaError_t launch_across(const T* X, size_t ldx, signed char* Q, size_t ldq, float* scale, size_t lines, size_t len, unsigned ranks, cudaStream_t s)
+{
+    const size_t strips = (len + 31) / 32;
     if (strips * ranks >= (1u << 31)) return cudaErrorNotSupported;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(strips * ranks));
@@ -222,7 +302,26 @@ cudaError_t launch_across(const T* X, size_t ldx, signed char* Q, size_t ldq, fl
     cfg.attrs = attr;
     cfg.numAttrs = 2;
     count_launch();
-    return cudaLaunchKernelEx(&cfg, quantize_across_kernel<T, V, KEEP>, X, ldx, Q, ldq, scale, lines, len);
+    return cudaLaunchKernelEx(&cfg, quantize_across_kernel<T, KEEP>, X, ldx, Q, ldq, scale, lines, len);
+}
+
+template <typename T, int V, int COLS>
+cudaError_t launch_across_passes(const T* X, size_t ldx, signed char* Q, size_t ldq, float* scale, size_t lines, size_t len, cudaStream_t s)
+{
+    const size_t strips = (len + COLS * V - 1) / (COLS * V), at_least = 8 * (32 / COLS);
+    if (strips >= (1u << 31)) return cudaErrorNotSupported;
+    // Blocks of lines: four CTAs per SM, 64 blocks at most (every CTA of the second pass reads their maxima).
+    size_t blocks = ((size_t)sm_count() * 4 + strips - 1) / strips;
+    blocks = std::min(std::min<size_t>(blocks, 64), (lines + at_least - 1) / at_least);
+    unsigned* tops = nullptr;
+    cudaError_t e = ws_alloc(reinterpret_cast<void**>(&tops), blocks * len * sizeof(unsigned), s);
+    if (e != cudaSuccess) return e;
+    const dim3 grid((unsigned)strips, (unsigned)blocks);
+    e = launch_chained(across_max_kernel<T, V, COLS>, grid, 256, s, X, ldx, tops, lines, len);
+    if (e == cudaSuccess) e = launch_chained(across_quantize_kernel<T, V, COLS>, grid, 256, s, X, ldx, Q, ldq, (const unsigned*)tops, scale, lines, len);
+    count_launch(2);
+    const cudaError_t e2 = ws_free(tops, s);
+    return e == cudaSuccess ? e2 : e;
 }
 
 template <typename T>
@@ -230,9 +329,19 @@ cudaError_t quantize_typed(bool per_line, const T* X, size_t ldx, signed char* Q
 {
     constexpr int V = 16 / sizeof(T);
     if (!per_line) {
-        const bool vec = len % 4 == 0 && (reinterpret_cast<uintptr_t>(X) | ldx * sizeof(T)) % (4 * sizeof(T)) == 0 && (reinterpret_cast<uintptr_t>(Q) | ldq) % 4 == 0;
-        if (vec) return launch_across<T, 4, 64 / sizeof(T)>(X, ldx, Q, ldq, scale, lines, len, s);
-        return launch_across<T, 1, 64>(X, ldx, Q, ldq, scale, lines, len, s);
+        const size_t strips = (len + 31) / 32;
+        unsigned ranks = 1;
+        while (ranks < 8 && lines > (size_t)8 * ranks && (lines > (size_t)8 * 64 * ranks || strips * ranks < 2 * (size_t)sm_count())) ranks *= 2;
+        const bool vec = aligned16(X) && (ldx * sizeof(T)) % 16 == 0 && len % V == 0 && (reinterpret_cast<uintptr_t>(Q) | ldq) % V == 0;
+        // us, one kernel / two passes: 300 x 16000 BF16 12 / 14, 4096 x 1024 FP32 6.5 / 12, 4096 x 4096 FP32 24.2 / 24.6 (unaligned 25 / 45),
+        // 4096 x 11008 BF16 117 / 57 (unaligned 118 / 114).
+        if (!(vec && lines * len > (1u << 24))) {
+            if (lines <= (size_t)8 * 64 * ranks) return launch_across<T, 64>(X, ldx, Q, ldq, scale, lines, len, ranks, s);
+            if (lines <= (size_t)8 * 80 * ranks) return launch_across<T, 80>(X, ldx, Q, ldq, scale, lines, len, ranks, s);
+        }
+        if (vec && len >= 8 * V) return len >= 32 * V ? launch_across_passes<T, V, 32>(X, ldx, Q, ldq, scale, lines, len, s)
+                                                      : launch_across_passes<T, V, 8>(X, ldx, Q, ldq, scale, lines, len, s);
+        return launch_across_passes<T, 1, 32>(X, ldx, Q, ldq, scale, lines, len, s);
     }
     if (lines >= (1u << 31)) return cudaErrorNotSupported;
     count_launch();

@@ -49,6 +49,19 @@ def test_against_the_definition(kind, order, side, pad, off):
         assert bool((off_by <= s64 * (0.5 + 127 * 4 * U32)).all())
 
 
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+@pytest.mark.parametrize("pad,off", [(0, 0), (3, 5)])
+def test_scales_across_many_lines(kind, pad, off):
+    """More lines, or more elements, than a cluster keeps in registers: two passes, by 16-byte and by single accesses."""
+    for M, N in ((4500, 40), (4500, 264), (5200, 520), (9000, 17), (4097, 2304), (8200, 3), (2048, 8320)):
+        x, q = build("row", M, N, kind, pad, off, seed=M + N)
+        scale = torch.full((N + 8,), 5.0, device="cuda")
+        cb.check(call("row", "right", M, N, kind, x, q, scale, off_s=4), "quantize")
+        want_q, want_s = quantize_reference(x.op()[0], 0)
+        assert torch.equal(q.op()[0].cpu(), want_q) and torch.equal(scale[4:4 + N].cpu(), want_s), (M, N)
+        assert bool((q.buf[q.outside()] == 77).all()) and bool((scale[:4] == 5).all()) and bool((scale[4 + N:] == 5).all())
+
+
 @pytest.mark.parametrize("side", ["left", "right"])
 @pytest.mark.parametrize("kind", ["bf16", "f32"])
 def test_zero_tiny_and_non_finite_lines(side, kind):
