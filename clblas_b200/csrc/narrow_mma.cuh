@@ -2,13 +2,16 @@
 // orthogonalisation).  Both are  D[u, v] = sum_k P[u, k] * Q[v, k]  with P stored U x K and Q stored V x K, k contiguous (or, for Q, v contiguous:
 // the MN-major form of the instruction); the epilogue is a functor.
 //
-// narrow_persistent_kernel: one CTA (or one pair of CTAs, tcgen05.mma.cta_group::2) per SM (pair of SMs) walks over output
-// tiles.  10 warps: warp 0 loads slabs of 128 bytes along k with TMA into a ring, warp 1 owns tensor memory and issues the
-// MMAs, warps 2-9 are the epilogue.  Two accumulators in tensor memory, so the epilogue of a tile runs under the products of the next.
+// narrow_persistent_kernel: pairs of CTAs (tcgen05.mma.cta_group::2, one CTA per SM) walk over output tiles of 256 rows.  10 warps: warp
+// 0 loads slabs of 128 bytes along k with TMA into a ring, warp 1 owns tensor memory and issues the MMAs, warps 2-9 are the
+// epilogue.  Two accumulators in tensor memory, so the epilogue of a tile runs under the products of the next.  Bound by what L2
+// feeds the SMs (about 13 TB/s measured; a 256 x 256 tile moves 64 KB per slab) and, over seconds, by the power cap: 8-bit 8192^3
+// 318 to 350 us alone, 402 to 416 us back to back (cuBLAS on the same GPU 377 and 439); FP16 gram product 4096 x 16384 182 to 205 us.
 //
 // narrow_split_kernel: for products with fewer tiles than SMs.  The k range of a tile is cut over the CTAs of a cluster; the
 // partial accumulators meet in distributed shared memory (each rank sums a slice of the columns, in rank order, so
-// results do not depend on timing), then the same epilogue runs on the slices.  No workspace, no second launch.
+// results do not depend on timing), then the same epilogue runs on the slices.  No workspace, no second launch.  Bound by latency
+// (launch 2 us, first load 0.7, barriers and exchange 2, epilogue 1) or, for few tokens, by reading the weights.
 //
 // Every wait on an mbarrier is bounded (tma_pipeline.cuh).  A CTA whose wait ran out leaves its loops and still takes part in
 // the cluster barriers, so its peers end too.
@@ -438,23 +441,20 @@ __device__ __forceinline__ void read_chunk(float (&x)[4][4][2], uint32_t taddr)
 
 template <int BN, int CG>
 constexpr int stage_bytes() { return (BM + BN / CG) * SLAB_BYTES; }
-template <int BN, int CG>
-constexpr int persistent_stages()
-{
-    return (232448 - 1024 - 512) / stage_bytes<BN, CG>();
-}
-template <int BN, int CG>
-constexpr int persistent_smem() { return persistent_stages<BN, CG>() * stage_bytes<BN, CG>() + 1024 + 512; }
+template <int BN>
+constexpr int persistent_stages() { return (232448 - 1024 - 512) / stage_bytes<BN, 2>(); }
+template <int BN>
+constexpr int persistent_smem() { return persistent_stages<BN>() * stage_bytes<BN, 2>() + 1024 + 512; }
 
 // ---------------------------------------------------------------------------------------------------------------------
 // Persistent kernel
 // ---------------------------------------------------------------------------------------------------------------------
 
-template <int KIND, int BN, int CG, bool QMN, class Epi>
+template <int KIND, int BN, bool QMN, class Epi>
 __global__ void __launch_bounds__(THREADS, 1)
 narrow_persistent_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__ CUtensorMap mapQ, const Shape s, const Epi epi)
 {
-    constexpr int STAGES = persistent_stages<BN, CG>(), STAGE = stage_bytes<BN, CG>();
+    constexpr int CG = 2, STAGES = persistent_stages<BN>(), STAGE = stage_bytes<BN, CG>();
     constexpr uint32_t TMEM_COLS = 2 * BN > 256 ? 512 : 256;          // two accumulators; a power of two
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -465,7 +465,7 @@ narrow_persistent_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
 
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const uint32_t rank = CG == 2 ? cluster_ctarank() : 0;
+    const uint32_t rank = cluster_ctarank();
     const unsigned group = blockIdx.x / CG, groups = gridDim.x / CG;
     const unsigned total = s.tiles * s.batch;
     const int nk = (int)((s.K + slab_k(KIND) - 1) / slab_k(KIND));
@@ -486,7 +486,7 @@ narrow_persistent_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_
     if (warp == 1) tmem_alloc<CG>(tmem_slot, TMEM_COLS);
     tc_fence_before();
     __syncthreads();
-    if (CG == 2) cluster_sync();
+    cluster_sync();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     pdl_launch_dependents();
@@ -505,8 +505,7 @@ narrow_persistent_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_
                     const int slot = it % STAGES;
                     if (it >= STAGES && !mbar_wait(&empty[slot], ((it / STAGES) - 1) & 1)) { ok = false; break; }
                     // A pair's loads are all counted on the first CTA's barrier, which expects both halves.
-                    uint32_t bar = smem_u32(&full[slot]);
-                    if (CG == 2) bar = map_shared(bar, 0);
+                    const uint32_t bar = map_shared(smem_u32(&full[slot]), 0);
                     if (rank == 0) mbar_expect_tx(&full[slot], CG * STAGE);
                     load_slab<KIND, BN, CG, QMN>(smem + slot * STAGE, &mapP, &mapQ, kt, u0, v0, (int)z, bar);
                 }
@@ -554,10 +553,7 @@ narrow_persistent_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_
                 if (c == CHUNKS - 1) {                        // accumulator read: hand it back
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) {
-                        if (CG == 2) mbar_arrive_cluster(map_shared(smem_u32(&acc_empty[a]), 0));
-                        else mbar_arrive(&acc_empty[a]);
-                    }
+                    if (lane == 0) mbar_arrive_cluster(map_shared(smem_u32(&acc_empty[a]), 0));
                 }
                 epi.chunk(st, pre, s, z, u0, v0 + c * 32, c + 1 < CHUNKS ? v0 + (c + 1) * 32 : ~0u, part_of(s, u0, v0 + c * 32), x);
             }
@@ -567,7 +563,7 @@ narrow_persistent_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_
     __syncwarp();
     tc_fence_before();
     __syncthreads();
-    if (CG == 2) cluster_sync();
+    cluster_sync();
     tc_fence_after();
     if (warp == 1) tmem_free<CG>(tmem, TMEM_COLS);
 }
@@ -791,11 +787,12 @@ cudaError_t launch(Kernel kernel, unsigned grid, unsigned cluster, int smem, cud
     return e;
 }
 
-template <int KIND, int BN, int CG, bool QMN, class Epi>
+template <int KIND, int BN, bool QMN, class Epi>
 cudaError_t run_persistent(const Operand& p, const Operand& q, Shape s, const Epi& epi, cudaStream_t st)
 {
-    auto kernel = narrow_persistent_kernel<KIND, BN, CG, QMN, Epi>;
-    constexpr int smem = persistent_smem<BN, CG>();
+    constexpr int CG = 2;
+    auto kernel = narrow_persistent_kernel<KIND, BN, QMN, Epi>;
+    constexpr int smem = persistent_smem<BN>();
     static DeviceOnce once;
     cudaError_t e = once.run([&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); });
     if (e != cudaSuccess) return e;
@@ -877,10 +874,10 @@ template <int KIND, bool QMN, class Epi>
 cudaError_t run_planned(const Operand& p, const Operand& q, const Shape& s, const Epi& epi, cudaStream_t st)
 {
     const Plan plan = choose_plan(s.U, s.V, s.K, s.batch, s.tri, KIND, Epi::kHeavy);
-    if (plan.pairs == 256) return run_persistent<KIND, 256, 2, QMN, Epi>(p, q, s, epi, st);
-    if (plan.pairs == 128) return run_persistent<KIND, 128, 2, QMN, Epi>(p, q, s, epi, st);
+    if (plan.pairs == 256) return run_persistent<KIND, 256, QMN, Epi>(p, q, s, epi, st);
+    if (plan.pairs == 128) return run_persistent<KIND, 128, QMN, Epi>(p, q, s, epi, st);
     if constexpr (KIND == KIND_I8)
-        if (plan.pairs == 192) return run_persistent<KIND, 192, 2, QMN, Epi>(p, q, s, epi, st);
+        if (plan.pairs == 192) return run_persistent<KIND, 192, QMN, Epi>(p, q, s, epi, st);
     return run_split_by<KIND, 128, QMN, Epi>(plan.split, p, q, s, epi, st);
 }
 

@@ -5,7 +5,12 @@
 //
 // On the smaller side n of the matrix (n <= m) a step is three products: the Gram matrix (symmetric, n^2 m operations), its
 // square (symmetric, n^3) and the update (2 n^2 m).  All run on the FP16 tensor-core tiles of narrow_mma.cuh, the symmetric ones on
-// the tiles of one triangle, each result stored at both places.
+// the tiles of one triangle, each result stored at both places.  (Matrices up to 128 x 2048 take one kernel instead of the
+// chain: orthogonalize_small.cu.)
+//
+// Measured, five steps: 4096 x 16384 BF16 3.65 ms alone, 4.2 ms back to back under the power cap (Gram 205 us, square 61, update 410: the
+// tiles without their epilogues 329, the rest is the 8 bytes an element that X costs to read and write); twelve 768 x 768 FP32 265 us
+// (15, 17, 29 us a step); two 2601 x 1003 257 us; 256 x 1024 98 us, of which launches and first loads are most.
 //
 // What is kept in how many bits, and why:
 //   * X is a pair of FP16 numbers, hi + lo (22 bits); a X uses the pair, the products use hi.  Singular values far below the
