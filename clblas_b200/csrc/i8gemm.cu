@@ -325,6 +325,7 @@ cudaError_t i8gemm_typed(const I8GemmProblem& p, cudaStream_t s)
 cudaError_t i8gemm(const I8GemmProblem& p, cudaStream_t s)
 {
     set_last_kernel("i8gemm_tcgen05");
+    set_last_variant("i8gemm_tcgen05");
     switch (p.type) {
         case clblasB200Float32: return i8gemm_typed<float>(p, s);
         case clblasB200Float16: return i8gemm_typed<__half>(p, s);

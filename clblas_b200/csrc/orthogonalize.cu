@@ -466,7 +466,6 @@ cudaError_t orthogonalize_typed(const OrthProblem& p, cudaStream_t s)
 
 cudaError_t orthogonalize(const OrthProblem& p, cudaStream_t s)
 {
-    set_last_kernel("orthogonalize_tcgen05");
     switch (p.type) {
         case clblasB200Float32: return orthogonalize_typed<float>(p, s);
         case clblasB200Float16: return orthogonalize_typed<__half>(p, s);

@@ -482,8 +482,10 @@ clblasStatus clblasB200I8gemm(
  *      its own norm).  beta == 0 never reads O.  A G that holds a NaN or an infinity gives NaN everywhere.  The iteration
  *      runs in FP16 with scale factors that leave room for singular values of X up to 16 and for |b| s^2 + |c| s^4 up to 255
  *      at singular values s; coefficients that drive X further overflow.
- *      G and O may be the same buffer, and matrices of G may overlap; matrices of O may not.
- *      Workspace (from the library's pool): about 6 bytes per element of G and 4 per element of the smaller square.
+ *      O may be G itself (BF16, same offset, pitch and stride); they may not overlap otherwise.  Matrices of G may overlap
+ *      one another (strideG 0: one gradient), matrices of O may not.
+ *      Workspace (from the library's pool): about 6 bytes per element of G and 4 per element of the smaller square; none up to
+ *      128 x 2048.
  *      Checks: G (A's status codes), O (C's; clblasInvalidLeadDimC also for a stride that makes its matrices overlap). */
 clblasStatus clblasB200Orthogonalize(
     clblasOrder order, size_t M, size_t N, size_t batchCount, unsigned steps, const float* coefficients, float alpha,

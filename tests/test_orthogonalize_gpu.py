@@ -187,3 +187,52 @@ def test_refusals():
     with pytest.raises(ValueError):
         go(steps=2, co=[(1.0, 2.0, 3.0)])
     assert cb.lib.clblasB200DeviceFault() == 0
+
+
+# The single kernel for small matrices: clusters of 1, 2, 4, 8 CTAs, widths of 64 to 256 columns per CTA, the sizes just beyond it.
+SMALL = [(1, 64), (64, 64), (65, 65), (128, 128), (33, 257), (100, 500), (128, 640), (127, 1025), (90, 1600), (128, 2048), (128, 2049), (129, 2048)]
+
+
+@pytest.mark.parametrize("n,m", SMALL)
+@pytest.mark.parametrize("tall", [False, True])
+def test_small_sizes(n, m, tall):
+    Problem("row", *((m, n) if tall else (n, m)), kind="f32" if n % 2 else "bf16", seed=n + m).check()
+
+
+@pytest.mark.parametrize("order", ["row", "col"])
+@pytest.mark.parametrize("M,N,batch", [(70, 300, 5), (300, 70, 5), (120, 900, 17), (50, 60, 150)])
+@pytest.mark.parametrize("kind,pad,off,gap", [("f32", 0, 0, 0), ("f32", 3, 5, 11), ("bf16", 8, 8, 64), ("f16", 2, 2, 6), ("bf16", 1, 3, 5)])
+def test_small_batches_and_layouts(order, M, N, batch, kind, pad, off, gap):
+    Problem(order, M, N, batch=batch, kind=kind, pad=pad, off=off, gap=gap, seed=4).check(alpha=-0.02, beta=0.99)
+
+
+@pytest.mark.parametrize("steps,coefficients", [(1, None), (2, None), (64, [(1.5, -0.5, 0.0)] * 64), (3, [(1.5, -0.5, 0.0), (3.4445, -4.775, 2.0315), (1.875, -1.25, 0.375)])])
+@pytest.mark.parametrize("M,N", [(100, 260), (260, 100)])
+def test_small_steps_and_coefficients(steps, coefficients, M, N):
+    Problem("row", M, N, seed=5).check(steps, coefficients, alpha=2.0)
+
+
+def test_small_is_deterministic_on_streams_and_in_graphs():
+    ps = [Problem("row", 100, 500 + 300 * i, batch=3, seed=20 + i) for i in range(3)]
+    want = []
+    for p in ps:
+        cb.check(p.call(), "alone")
+        want.append(p.o.op().clone())
+        p.o.buf.zero_()
+    streams = [torch.cuda.Stream() for _ in ps]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for p, s in zip(ps, streams):
+            cb.check(p.call(queues=[s]), "streams")
+    torch.cuda.synchronize()
+    assert all(torch.equal(p.o.op(), w) for p, w in zip(ps, want))
+    p, s = ps[0], streams[0]
+    p.o.buf.zero_()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        cb.check(p.call(), "captured")
+        cb.check(p.call(), "captured")
+    g.replay()
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(p.o.op(), want[0]) and cb.lib.clblasB200DeviceFault() == 0
