@@ -826,13 +826,15 @@ cudaError_t run_split(const Operand& p, const Operand& q, Shape s, const Epi& ep
 //           come in blocks of 64 per CTA, triangles in blocks of 128)
 //   split:  128 x 128 tiles, one per cluster of `split` CTAs, which share k and the epilogue's columns
 // The plan with the shortest estimate is taken.  The estimates, in us, are fitted to all plans measured on twelve FP16 shapes from
-// 100 x 130 to 2048 x 8192; on those and on thirteen 8-bit shapes the plan taken was within 7 % of the best:
+// 100 x 130 to 2048 x 8192; on thirteen 8-bit shapes from 160 x 4096 x 4096 to 8192 x 1024 x 8192 the plan taken was within 6 % of
+// the best:
 //   a launch and its end                 3, persistent 5
 //   a slab of k, 128 x 128 tiles         0.30                            1 round of 136 tiles, 128 slabs: 46.7
 //   a slab of k, 256 x 256               0.30 for a lone tile, 0.37 with all SMs at it, 0.36 to 0.45 in later rounds, when
 //                                        the epilogues (0.45: `heavy` ones, that read as much as they write) share L2 with the loads
 //   a slab of k, 256 x 128               0.30, later 0.37
-//   an epilogue                          128 x 128: 5.0, 4.6, 4.2 with 1, 2, 4 CTAs at it (heavy: 6.3, 5.6, 4.5); 256 x 256: 5.0 (8.5), 256 x 128: 5.0 (7.0) for each round, 0.7 of it exposed in the first
+//   an epilogue                          128 x 128: 5.0, 4.6, 4.2 with 1, 2, 4 CTAs at it (heavy: 6.3, 5.6, 4.5); 256 x 256: 5.0
+//                                        (8.5); 256 x 128: 5.0 (7.0) a round, 0.7 of it in the first
 // A round of a persistent kernel takes the longer of its slabs and the epilogue before; clusters of 4 fill 128 SMs, clusters of 8 (never the
 // best here) fewer.
 struct Plan { unsigned pairs, split; };               // one of the two is 0
