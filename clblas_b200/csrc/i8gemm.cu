@@ -38,7 +38,9 @@ struct EpiScaled {
     static constexpr bool kHeavy = sizeof(T) == 4;
     struct State { float factor[4]; };
     template <int G> struct Pre { Bits16<G> c; };
-    const float* su;                // scales of the rows u and the columns v; nullptr: ones
+    // Scales of the rows u and the columns v; nullptr: ones.  Read by ordinary loads after pdl_wait() and not as constants (__ldg): the
+    // quantisation before may still write them while this kernel is already resident, next to a product that has the old ones cached.
+    const float* su;
     const float* sv;
     float alpha, beta;
     T* C;
@@ -50,7 +52,7 @@ struct EpiScaled {
     {
         const unsigned u = u0 + (threadIdx.x & 31) / 4;
 #pragma unroll
-        for (int g = 0; g < 4; g++) st.factor[g] = su && u + 8 * g < s.U ? alpha * __ldg(su + u + 8 * g) : alpha;
+        for (int g = 0; g < 4; g++) st.factor[g] = su && u + 8 * g < s.U ? alpha * su[u + 8 * g] : alpha;
     }
     template <int G>
     __device__ void fetch(Pre<G>& p, const Shape& s, unsigned, unsigned u0, unsigned v0) const
@@ -67,7 +69,7 @@ struct EpiScaled {
 #pragma unroll
         for (int k = 0; k < G; k++) {
             const unsigned v = v0 + 8 * k + 2 * q;
-            const float w0 = sv && v < s.V ? __ldg(sv + v) : 1.f, w1 = sv && v + 1 < s.V ? __ldg(sv + v + 1) : 1.f;
+            const float w0 = sv && v < s.V ? sv[v] : 1.f, w1 = sv && v + 1 < s.V ? sv[v + 1] : 1.f;
 #pragma unroll
             for (int g = 0; g < 4; g++) {
                 x[g][k][0] = x[g][k][0] * st.factor[g] * w0;

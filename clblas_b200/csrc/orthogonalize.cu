@@ -99,9 +99,10 @@ __global__ void __launch_bounds__(256) sum_squares_kernel(const T* __restrict__ 
 }
 
 // X0 = G / (|G| + eps), times SX, as hi + lo; FLIP: transposed on the way (G has more lines than elements per line).
-// A matrix that holds a NaN or an infinity becomes NaN everywhere.  64 lines x 64 elements per CTA.  Bound by memory.
+// A matrix that holds a NaN or an infinity becomes NaN everywhere.  64 lines x 64 elements per CTA.  Bound by memory.  (`part` is written
+// while this kernel is already resident: no `__restrict__`, which would allow loads as of constants.)
 template <typename T, bool VEC, bool FLIP>
-__global__ void __launch_bounds__(256) split_kernel(const T* __restrict__ G, size_t lines, size_t len, size_t ld, size_t stride, const double* __restrict__ part,
+__global__ void __launch_bounds__(256) split_kernel(const T* G, size_t lines, size_t len, size_t ld, size_t stride, const double* part,
                                                     int parts, __half* __restrict__ hi, __half* __restrict__ lo, size_t ldx, size_t stride_x,
                                                     u64* __restrict__ sums, int sums_pitch, unsigned tiles_len)
 {

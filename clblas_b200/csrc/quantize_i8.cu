@@ -5,6 +5,9 @@
 // infinity gets s = NaN, q = 0: the product with it is NaN, as the product with the line itself would be.
 //
 // Bound by memory: each element is read once and one byte written.
+//
+// The kernels start while the one before them, which may write X, still runs.  X is therefore no `const __restrict__` pointer: that
+// would allow loads through the cache for constants, which may be taken ahead of the wait.
 #include "common.h"
 #include "tma_pipeline.cuh"
 
@@ -72,7 +75,7 @@ __device__ __forceinline__ void put(signed char* q, const Word<T, V>& w, const L
 // One line (contiguous elements, one scale) per CTA of THREADS threads; V elements per access.  A thread keeps its first KEEP
 // accesses in registers between the maximum and the quantisation; longer lines are read again from there on.
 template <typename T, int THREADS, int V, int KEEP>
-__global__ void __launch_bounds__(THREADS) quantize_lines_kernel(const T* __restrict__ X, size_t ldx, signed char* __restrict__ Q, size_t ldq,
+__global__ void __launch_bounds__(THREADS) quantize_lines_kernel(const T* X, size_t ldx, signed char* __restrict__ Q, size_t ldq,
                                                                  float* __restrict__ scale, size_t len)
 {
     typedef Word<T, V> W;
@@ -120,7 +123,7 @@ __global__ void __launch_bounds__(THREADS) quantize_lines_kernel(const T* __rest
 // thread keeps its elements in registers, the maxima meet in distributed shared memory and every CTA quantises its own lines:
 // one launch, each element read once.  KEEP elements a thread: 64, or the 80 that two CTAs per SM have room for when that saves a pass.
 template <typename T, int KEEP>
-__global__ void __launch_bounds__(256) quantize_across_kernel(const T* __restrict__ X, size_t ldx, signed char* __restrict__ Q, size_t ldq,
+__global__ void __launch_bounds__(256) quantize_across_kernel(const T* X, size_t ldx, signed char* __restrict__ Q, size_t ldq,
                                                               float* __restrict__ scale, size_t lines, size_t len)
 {
     __shared__ unsigned tops[8][32], joined[32];
@@ -196,7 +199,7 @@ struct AcrossBlock {
 };
 
 template <typename T, int V, int COLS>
-__global__ void __launch_bounds__(256) across_max_kernel(const T* __restrict__ X, size_t ldx, unsigned* __restrict__ tops, size_t lines, size_t len)
+__global__ void __launch_bounds__(256) across_max_kernel(const T* X, size_t ldx, unsigned* __restrict__ tops, size_t lines, size_t len)
 {
     typedef AcrossBlock<T, V, COLS> B;
     __shared__ unsigned per_warp[8][COLS * V];
@@ -236,8 +239,8 @@ __global__ void __launch_bounds__(256) across_max_kernel(const T* __restrict__ X
 }
 
 template <typename T, int V, int COLS>
-__global__ void __launch_bounds__(256) across_quantize_kernel(const T* __restrict__ X, size_t ldx, signed char* __restrict__ Q, size_t ldq,
-                                                              const unsigned* __restrict__ tops, float* __restrict__ scale, size_t lines, size_t len)
+__global__ void __launch_bounds__(256) across_quantize_kernel(const T* X, size_t ldx, signed char* __restrict__ Q, size_t ldq,
+                                                              const unsigned* tops, float* __restrict__ scale, size_t lines, size_t len)
 {
     typedef AcrossBlock<T, V, COLS> B;
     __shared__ unsigned joined[COLS * V];
