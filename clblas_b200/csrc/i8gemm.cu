@@ -48,7 +48,7 @@ struct EpiScaled {
     bool trans;                     // element (u, v) at C[v * ld + u] instead of C[u * ld + v]
     int align;                      // of C's lines: 16, 4 or 2 bytes (16-bit C); 8-byte accesses allowed when 8 or more (32-bit C)
 
-    __device__ void begin(State& st, const Shape& s, unsigned, unsigned u0) const
+    __device__ void begin(State& st, const Shape& s, unsigned, unsigned u0, unsigned) const
     {
         const unsigned u = u0 + (threadIdx.x & 31) / 4;
 #pragma unroll

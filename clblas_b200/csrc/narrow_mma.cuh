@@ -222,7 +222,7 @@ __host__ __device__ inline void tile_coords(const Shape& s, unsigned t, unsigned
 // Epilogue.  A warp finishes chunks of 32 rows x 8 G columns, held as fragments x[g][k][e]: row 8 g + lane / 4, column
 // 8 k + 2 (lane % 4) + e.  What a functor has:
 //   kHeavy        reads as much as it writes (for choose_plan)
-//   begin()       per thread and tile
+//   begin()       per thread and tile; u0, v0: where the warp's first chunk begins (of all its tiles one warp has both 0)
 //   Pre, fetch()  what a chunk needs besides the accumulators, requested one chunk ahead
 //   chunk()       computes and stores (where: part_of()); requests the next chunk's (at column v_next, ~0u: none) as soon as its own is used
 //   end()         per thread and tile
@@ -541,7 +541,7 @@ narrow_persistent_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_
             constexpr int CHUNKS = BN / 32 / 2;               // per half
             const unsigned v0 = tv * BN + half * CHUNKS * 32;
             typename Epi::State st;
-            epi.begin(st, s, z, u0);
+            epi.begin(st, s, z, u0, v0);
             typename Epi::template Pre<4> pre;
             epi.fetch(pre, s, z, u0, v0);
             if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[a], (n >> 1) & 1))) break;
@@ -659,7 +659,7 @@ narrow_split_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_const
     typename Epi::template Pre<G> pre;
     bool ok = true;
     if (warp >= 2) {
-        epi.begin(st, s, z, u0);
+        epi.begin(st, s, z, u0, v_own);
         if (finishes) epi.fetch(pre, s, z, u0, v_own);
         ok = __all_sync(0xffffffffu, mbar_wait(acc_full, 0));
         tc_fence_after();

@@ -23,7 +23,8 @@
 //   * t comes from the sum of the squares of X, gathered in 64-bit integers (units of 2^-24), so the order of the atomic additions does
 //     not change it.  Any t gives the same polynomial; it only has to be near.
 //   * Accumulators and everything between accumulator and store are FP32.  X is held times 2^12, A and P times 2^8, so that the
-//     entries of large matrices (about 1/sqrt(m)) stay far above FP16's smallest numbers.
+//     entries of large matrices (about 1/sqrt(m)) stay far above FP16's smallest numbers, and times a power of two for each matrix where
+//     the whole matrix is small (orthogonalize.cuh).  768 x 768, |G|_F = 1e-15: 32 % off without that power, 3.4e-4 with it.
 // The result is good to about 1e-3 and is therefore given in BF16 only.
 #include "orthogonalize.cuh"
 
@@ -98,13 +99,13 @@ __global__ void __launch_bounds__(256) sum_squares_kernel(const T* __restrict__ 
     }
 }
 
-// X0 = G / (|G| + eps), times SX, as hi + lo; FLIP: transposed on the way (G has more lines than elements per line).
+// X0 = G / (|G| + eps), times 2^e SX, as hi + lo; FLIP: transposed on the way (G has more lines than elements per line).
 // A matrix that holds a NaN or an infinity becomes NaN everywhere.  64 lines x 64 elements per CTA.  Bound by memory.  (`part` is written
 // while this kernel is already resident: no `__restrict__`, which would allow loads as of constants.)
 template <typename T, bool VEC, bool FLIP>
 __global__ void __launch_bounds__(256) split_kernel(const T* G, size_t lines, size_t len, size_t ld, size_t stride, const double* part,
                                                     int parts, __half* __restrict__ hi, __half* __restrict__ lo, size_t ldx, size_t stride_x,
-                                                    u64* __restrict__ sums, int sums_pitch, unsigned tiles_len)
+                                                    u64* __restrict__ sums, int* __restrict__ exps, int sums_pitch, unsigned tiles_len)
 {
     __shared__ float factors[2];
     __shared__ float tile[FLIP ? 64 : 1][65];
@@ -129,8 +130,12 @@ __global__ void __launch_bounds__(256) split_kernel(const T* G, size_t lines, si
         for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
         if (threadIdx.x == 0) {
             double square;
-            norm_factors(sqrt(sum), factors[0], factors[1], square);
-            if (blockIdx.x == 0) sums[(size_t)z * sums_pitch] = (u64)(square * SUM_UNIT);
+            int e;
+            norm_factors(sqrt(sum), factors[0], factors[1], square, e);
+            if (blockIdx.x == 0) {
+                sums[(size_t)z * sums_pitch] = (u64)(square * SUM_UNIT);
+                exps[(size_t)z * sums_pitch] = e;
+            }
         }
     }
     __syncthreads();
@@ -183,11 +188,15 @@ __global__ void __launch_bounds__(256) split_kernel(const T* G, size_t lines, si
 
 // ---- epilogues ----------------------------------------------------------------------------------------------------------
 
-// The shift from the gathered sum of squares.
-__device__ __forceinline__ float shift_of(const u64* sums, size_t at, float inv_n)
-{
-    return shift((float)((double)__ldcg(sums + at) * (1.0 / SUM_UNIT)) * inv_n);       // past L1: a neighbour is added to meanwhile
-}
+// What the Gram product of a step finds and leaves for the others.
+struct Sizes {
+    const u64* sums; int* exps;                            // sum of squares and exponent of every matrix before the step, `pitch` apart
+    float4* factors;                                       // of the step: b, f, w, g (StepFactors)
+    int pitch;
+    float n, a, b, c;
+    bool last;
+    float scale;
+};
 
 // The workspaces have a pitch of a multiple of 8 elements: every row piece is aligned.
 __device__ __forceinline__ uint16_t* bits(__half* p) { return reinterpret_cast<uint16_t*>(p); }
@@ -198,9 +207,21 @@ struct EpiGram {                                           // A <- X X' - t I
     struct State { float t; };
     template <int G> struct Pre {};
     __half* A; size_t ld, stride;
-    const u64* sums; int pitch;
-    float inv_n;
-    __device__ void begin(State& st, const Shape&, unsigned z, unsigned) const { st.t = SA * shift_of(sums, (size_t)z * pitch, inv_n); }
+    Sizes sizes;
+    __device__ void begin(State& st, const Shape&, unsigned z, unsigned u0, unsigned v0) const
+    {
+        const size_t at = (size_t)z * sizes.pitch;         // read past L1: a neighbour is written meanwhile
+        const float mean = (float)((double)__ldcg(sizes.sums + at) * (1.0 / SUM_UNIT)) * (1.f / sizes.n);
+        const int e = __ldcg(sizes.exps + at);
+        const float t = shift(mean, e);
+        st.t = SA * t;
+        // Once for a matrix: evaluated by every tile of the products that need them they took 0.35 us a kernel.
+        if (u0 == 0 && v0 == 0 && (threadIdx.x & 31) == 0) {
+            const StepFactors k = step_factors(mean * sizes.n, t, e, sizes.a, sizes.b, sizes.c, sizes.last, sizes.scale);
+            sizes.factors[at] = make_float4(k.b, k.f, k.w, k.g);
+            sizes.exps[at + 1] = k.next;
+        }
+    }
     template <int G> __device__ void fetch(Pre<G>&, const Shape&, unsigned, unsigned, unsigned) const {}
     template <int G>
     __device__ void chunk(State& st, Pre<G>&, const Shape& s, unsigned z, unsigned u0, unsigned v0, unsigned, int where, float (&x)[4][G][2]) const
@@ -224,14 +245,18 @@ struct EpiGram {                                           // A <- X X' - t I
     __device__ void end(State&, unsigned, unsigned) const {}
 };
 
-struct EpiSquare {                                         // P <- (b + 2 c t) A + c A^2
+struct EpiSquare {                                         // P <- (b + 2 c t) A + c A^2, times 2^p
     static constexpr bool kHeavy = false;
-    struct State { float b; };
+    struct State { float b, f; };
     template <int G> struct Pre { Bits16<G> a; };
     const __half* A; __half* P; size_t ld, stride;
-    const u64* sums; int pitch;
-    float inv_n, b, c;
-    __device__ void begin(State& st, const Shape&, unsigned z, unsigned) const { st.b = b + 2.f * c * shift_of(sums, (size_t)z * pitch, inv_n); }
+    const float4* factors; int pitch;
+    __device__ void begin(State& st, const Shape&, unsigned z, unsigned, unsigned) const
+    {
+        const float4 k = __ldcg(factors + (size_t)z * pitch);
+        st.b = k.x;
+        st.f = k.y;
+    }
     template <int G>
     __device__ void fetch(Pre<G>& p, const Shape& s, unsigned z, unsigned u0, unsigned v0) const
     {
@@ -241,14 +266,13 @@ struct EpiSquare {                                         // P <- (b + 2 c t) A
     __device__ void chunk(State& st, Pre<G>& p, const Shape& s, unsigned z, unsigned u0, unsigned v0, unsigned v_next, int where, float (&x)[4][G][2]) const
     {
         rows_to_fragments<G>(p.a, v0, s.V, PADDED);
-        const float f = c / SA;
         Bits16<G> o;
 #pragma unroll
         for (int g = 0; g < 4; g++)
 #pragma unroll
             for (int k = 0; k < G; k++) {
                 const float2 a = unpack(p.a.h[g][k]);
-                o.h[g][k] = pack(fmaf(st.b, a.x, f * x[g][k][0]), fmaf(st.b, a.y, f * x[g][k][1]));
+                o.h[g][k] = pack(fmaf(st.b, a.x, st.f * x[g][k][0]), fmaf(st.b, a.y, st.f * x[g][k][1]));
             }
         if (v_next != ~0u) fetch<G>(p, s, z, u0, v_next);
         if (where == PART_BELOW) store_columns16<G>(o, bits(P + z * stride), ld, u0, v0, s.U, s.V, PADDED);
@@ -257,58 +281,56 @@ struct EpiSquare {                                         // P <- (b + 2 c t) A
     __device__ void end(State&, unsigned, unsigned) const {}
 };
 
-// Common part of the two updates: y = (a + b t + c t^2) X + P X, times SX.  P is P, or A with factor b when c == 0.
+// Common part of the two updates: y = (a + b t + c t^2) X + P X.  P is P, or A with factor b when c == 0.
 struct UpdateTerm {
     const __half* hi; const __half* lo; size_t ld, stride;
-    const u64* sums; int pitch;
-    float inv_n, a, b, c;
+    const float4* factors; int pitch;
     template <int G> struct Pre { Bits16<G> h, l; };
+    struct Factors { float w, g; };                        // of X and of the product
     template <int G>
     __device__ void fetch(Pre<G>& p, const Shape& s, unsigned z, unsigned u0, unsigned v0) const
     {
         load_rows16<G>(p.h, bits(hi + z * stride), ld, u0, v0, s.U, s.V, PADDED);
         load_rows16<G>(p.l, bits(lo + z * stride), ld, u0, v0, s.U, s.V, PADDED);
     }
-    __device__ float coefficient(unsigned z) const
+    __device__ Factors of(unsigned z) const
     {
-        const float t = shift_of(sums, (size_t)z * pitch, inv_n);
-        return a + t * (b + c * t);
+        const float4 k = __ldcg(factors + (size_t)z * pitch);
+        return {k.z, k.w};
     }
-    // x <- scale * (coefficient X + P X)
     template <int G>
-    __device__ void add(Pre<G>& p, const Shape& s, unsigned v0, float coefficient, float scale, float (&x)[4][G][2]) const
+    __device__ void add(Pre<G>& p, const Shape& s, unsigned v0, const Factors& by, float (&x)[4][G][2]) const
     {
         rows_to_fragments<G>(p.h, v0, s.V, PADDED);
         rows_to_fragments<G>(p.l, v0, s.V, PADDED);
-        const float f = scale * ((c == 0.f ? b : 1.f) / SA), w = scale * coefficient;
 #pragma unroll
         for (int g = 0; g < 4; g++)
 #pragma unroll
             for (int k = 0; k < G; k++) {
                 const float2 h = unpack(p.h.h[g][k]), l = unpack(p.l.h[g][k]);
-                x[g][k][0] = fmaf(w, h.x + l.x, f * x[g][k][0]);
-                x[g][k][1] = fmaf(w, h.y + l.y, f * x[g][k][1]);
+                x[g][k][0] = fmaf(by.w, h.x + l.x, by.g * x[g][k][0]);
+                x[g][k][1] = fmaf(by.w, h.y + l.y, by.g * x[g][k][1]);
             }
     }
 };
 
 struct EpiUpdate {
     static constexpr bool kHeavy = true;
-    struct State { float a, sum; };
+    struct State { UpdateTerm::Factors by; float sum; };
     template <int G> using Pre = UpdateTerm::Pre<G>;
     UpdateTerm t;
     __half* hi; __half* lo;                                // lo may be the one that is read: each place is read, then written, by one thread
     u64* next;                                             // sums of the new X
-    __device__ void begin(State& st, const Shape&, unsigned z, unsigned) const
+    __device__ void begin(State& st, const Shape&, unsigned z, unsigned, unsigned) const
     {
-        st.a = t.coefficient(z);
+        st.by = t.of(z);
         st.sum = 0.f;
     }
     template <int G> __device__ void fetch(Pre<G>& p, const Shape& s, unsigned z, unsigned u0, unsigned v0) const { t.fetch<G>(p, s, z, u0, v0); }
     template <int G>
     __device__ void chunk(State& st, Pre<G>& p, const Shape& s, unsigned z, unsigned u0, unsigned v0, unsigned v_next, int, float (&x)[4][G][2]) const
     {
-        t.add<G>(p, s, v0, st.a, 1.f, x);
+        t.add<G>(p, s, v0, st.by, x);
         if (v_next != ~0u) fetch<G>(p, s, z, u0, v_next);
         const int lane = threadIdx.x & 31;
         Bits16<G> h, l;
@@ -345,14 +367,14 @@ struct EpiUpdate {
 
 struct EpiOut {                                            // O <- alpha X + beta O
     static constexpr bool kHeavy = true;
-    struct State { float a; };
+    struct State { UpdateTerm::Factors by; };
     template <int G> struct Pre { UpdateTerm::Pre<G> x; Bits16<G> o; };
     UpdateTerm t;
     uint16_t* O; size_t ldo, stride_o;                     // BF16
-    float alpha, beta;
+    float beta;                                            // (alpha is in the factors)
     bool flip;                                             // element (u, v) at O[v * ldo + u]
     int align;                                             // of O's lines
-    __device__ void begin(State& st, const Shape&, unsigned z, unsigned) const { st.a = t.coefficient(z); }
+    __device__ void begin(State& st, const Shape&, unsigned z, unsigned, unsigned) const { st.by = t.of(z); }
     template <int G>
     __device__ void fetch(Pre<G>& p, const Shape& s, unsigned z, unsigned u0, unsigned v0) const
     {
@@ -364,7 +386,7 @@ struct EpiOut {                                            // O <- alpha X + bet
     template <int G>
     __device__ void chunk(State& st, Pre<G>& p, const Shape& s, unsigned z, unsigned u0, unsigned v0, unsigned v_next, int, float (&x)[4][G][2]) const
     {
-        t.add<G>(p.x, s, v0, st.a, alpha / SX, x);
+        t.add<G>(p.x, s, v0, st.by, x);
         uint16_t* o = O + z * stride_o;
         if (beta != 0.f) {
             if (flip) columns_to_fragments<G>(p.o);
@@ -408,17 +430,19 @@ cudaError_t orthogonalize_typed(const OrthProblem& p, cudaStream_t s)
     // Blocks of the norm: about 8 pieces a thread, at most two blocks per SM over the batch.
     const size_t blocks = (p.lines * ((p.len + 7) / 8) + 2047) / 2048, most = std::max<size_t>(1, 2 * (size_t)sm_count() / batch);
     const size_t parts = std::min(blocks, most);
-    // workspace: hi (two of them, read and written in turn), lo, A, P, sums of squares, partial norms
-    const size_t x_bytes = up(batch * xs * 2, 256), a_bytes = up(batch * as * 2, 256), sum_bytes = up(batch * pitch * 8, 256);
+    // workspace: hi (two of them, read and written in turn), lo, A, P, sums of squares, exponents, factors, partial norms
+    const size_t x_bytes = up(batch * xs * 2, 256), a_bytes = up(batch * as * 2, 256), sum_bytes = up(batch * pitch * 8, 256), exp_bytes = up(batch * pitch * 4, 256), factor_bytes = up(batch * pitch * 16, 256);
     unsigned char* ws = nullptr;
-    cudaError_t e = ws_alloc(reinterpret_cast<void**>(&ws), 3 * x_bytes + 2 * a_bytes + sum_bytes + batch * parts * 8, s);
+    cudaError_t e = ws_alloc(reinterpret_cast<void**>(&ws), 3 * x_bytes + 2 * a_bytes + sum_bytes + exp_bytes + factor_bytes + batch * parts * 8, s);
     if (e != cudaSuccess) return e;
     __half* hi[2] = {reinterpret_cast<__half*>(ws), reinterpret_cast<__half*>(ws + x_bytes)};
     __half* lo = reinterpret_cast<__half*>(ws + 2 * x_bytes);
     __half* A = reinterpret_cast<__half*>(ws + 3 * x_bytes);
     __half* P = reinterpret_cast<__half*>(ws + 3 * x_bytes + a_bytes);
     u64* sums = reinterpret_cast<u64*>(ws + 3 * x_bytes + 2 * a_bytes);
-    double* part = reinterpret_cast<double*>(ws + 3 * x_bytes + 2 * a_bytes + sum_bytes);
+    int* exps = reinterpret_cast<int*>(ws + 3 * x_bytes + 2 * a_bytes + sum_bytes);
+    float4* factors = reinterpret_cast<float4*>(ws + 3 * x_bytes + 2 * a_bytes + sum_bytes + exp_bytes);
+    double* part = reinterpret_cast<double*>(ws + 3 * x_bytes + 2 * a_bytes + sum_bytes + exp_bytes + factor_bytes);
     const T* G = static_cast<const T*>(p.G) + p.offG;
 
     const size_t tl = (p.len + 63) / 64, tiles = tl * ((p.lines + 63) / 64);
@@ -430,33 +454,33 @@ cudaError_t orthogonalize_typed(const OrthProblem& p, cudaStream_t s)
             constexpr bool V = decltype(is_vec)::value, F = decltype(is_flip)::value;
             sum_squares_kernel<T, V><<<g1, 256, 0, s>>>(G, p.lines, (unsigned)p.len, p.ldg, p.strideG, part, sums, pitch);
             count_launch(2);
-            return launch_chained(split_kernel<T, V, F>, g2, 256, s, G, p.lines, p.len, p.ldg, p.strideG, (const double*)part, (int)parts, hi[0], lo, ldx, xs, sums, pitch, (unsigned)tl);
+            return launch_chained(split_kernel<T, V, F>, g2, 256, s, G, p.lines, p.len, p.ldg, p.strideG, (const double*)part, (int)parts, hi[0], lo, ldx, xs, sums, exps, pitch, (unsigned)tl);
         };
         if (vec) e = flip ? prepare(std::true_type{}, std::true_type{}) : prepare(std::true_type{}, std::false_type{});
         else     e = flip ? prepare(std::false_type{}, std::true_type{}) : prepare(std::false_type{}, std::false_type{});
     }
-    const float inv_n = 1.f / (float)n;
     for (int k = 0; k < p.steps && e == cudaSuccess; k++) {
         const float a = p.coeffs ? p.coeffs[3 * k] : 3.4445f, b = p.coeffs ? p.coeffs[3 * k + 1] : -4.7750f, c = p.coeffs ? p.coeffs[3 * k + 2] : 2.0315f;
+        const Sizes sizes{sums + k, exps + k, factors + k, pitch, (float)n, a, b, c, k + 1 == p.steps, p.alpha / SX};
         __half* x = hi[k & 1];
         const Operand ox{x, m, n, ldx, xs}, oa{A, n, n, ldn, as}, op{P, n, n, ldn, as};
         Shape sq = {};
         sq.U = sq.V = (unsigned)n; sq.K = (unsigned)m; sq.batch = (unsigned)batch; sq.tri = 1;
-        e = run_planned<KIND_F16, false>(ox, ox, sq, EpiGram{A, ldn, as, sums + k, pitch, inv_n}, s);
+        e = run_planned<KIND_F16, false>(ox, ox, sq, EpiGram{A, ldn, as, sizes}, s);
         if (e == cudaSuccess && c != 0.f) {
             sq.K = (unsigned)n;
-            e = run_planned<KIND_F16, false>(oa, oa, sq, EpiSquare{A, P, ldn, as, sums + k, pitch, inv_n, b, c}, s);
+            e = run_planned<KIND_F16, false>(oa, oa, sq, EpiSquare{A, P, ldn, as, factors + k, pitch}, s);
         }
         if (e != cudaSuccess) break;
         Shape up_ = {};
         up_.U = (unsigned)n; up_.V = (unsigned)m; up_.K = (unsigned)n; up_.batch = (unsigned)batch;
-        const UpdateTerm t{x, lo, ldx, xs, sums + k, pitch, inv_n, a, b, c};
+        const UpdateTerm t{x, lo, ldx, xs, factors + k, pitch};
         if (k + 1 < p.steps) {
             e = run_planned<KIND_F16, true>(c != 0.f ? op : oa, ox, up_, EpiUpdate{t, hi[(k + 1) & 1], lo, sums + k + 1}, s);
         } else {
             uint16_t* O = static_cast<uint16_t*>(p.O) + p.offO;
             const int align = line_alignment(O, p.ldo, batch > 1 ? p.strideO : 0);
-            e = run_planned<KIND_F16, true>(c != 0.f ? op : oa, ox, up_, EpiOut{t, O, p.ldo, p.strideO, p.alpha, p.beta, flip, align}, s);
+            e = run_planned<KIND_F16, true>(c != 0.f ? op : oa, ox, up_, EpiOut{t, O, p.ldo, p.strideO, p.beta, flip, align}, s);
         }
     }
     const cudaError_t e2 = ws_free(ws, s);

@@ -169,7 +169,8 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) orthogonalize_small_kernel(c
     cluster_sync();
     float f0, f1;
     double square;
-    norm_factors(sqrt(gathered(0.0)), f0, f1, square);
+    int e;                                                     // X is held times 2^e
+    norm_factors(sqrt(gathered(0.0)), f0, f1, square, e);
     const float per_mean = 1.f / (SX * SX * (float)p.n), mean0 = (float)(square / p.n);
 
     constexpr int MINE = SMALL_W / 64;                         // chunks per warp at most
@@ -239,7 +240,8 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) orthogonalize_small_kernel(c
         __syncwarp();
         cluster_sync();
         // ---- this rank's slice of A = X X' - t I, into every CTA ----
-        const float t = shift(step == 0 ? mean0 : gathered(0.f) * per_mean);
+        const bool last = step + 1 == p.steps;
+        const float mean = step == 0 ? mean0 : gathered(0.f) * per_mean, t = shift(mean, e);
 #pragma unroll
         for (int jj = 0; jj < (OWN + 1) / 2; jj++) {
             const int j = half + 2 * jj;
@@ -271,6 +273,7 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) orthogonalize_small_kernel(c
         __syncwarp();
         cluster_sync();
         // ---- P <- (b + 2 c t) A + c A^2 ----
+        StepFactors by;
         if (c != 0.f) {
             if (threadIdx.x == 0) {
                 proxy_fence();
@@ -283,8 +286,8 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) orthogonalize_small_kernel(c
                 umma_commit<1>(bar);
             }
             __syncwarp();
+            by = step_factors(mean * (float)p.n, t, e, a, b, c, last, p.alpha / SX);       // under the products
             wait_products();
-            const float ba = b + 2.f * c * t;
 #pragma unroll
             for (int i = 0; i < 2; i++) {
                 float x[4][4][2];
@@ -296,7 +299,7 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) orthogonalize_small_kernel(c
                     for (int k = 0; k < 4; k++) {
                         uint32_t* w = reinterpret_cast<uint32_t*>(A + slab_at(row0 + 8 * g, c0 + 8 * k + 2 * q));
                         const float2 v = unpack(*w);
-                        *w = pack(fmaf(ba, v.x, (c / SA) * x[g][k][0]), fmaf(ba, v.y, (c / SA) * x[g][k][1]));
+                        *w = pack(fmaf(by.b, v.x, by.f * x[g][k][0]), fmaf(by.b, v.y, by.f * x[g][k][1]));
                     }
             }
             tc_fence_before();
@@ -318,9 +321,9 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) orthogonalize_small_kernel(c
             umma_commit<1>(bar);
         }
         __syncwarp();
+        if (c == 0.f) by = step_factors(mean * (float)p.n, t, e, a, b, c, last, p.alpha / SX);
         wait_products();
-        const bool last = step + 1 == p.steps;
-        const float scale = last ? p.alpha / SX : 1.f, w = scale * (a + t * (b + c * t)), f = scale * ((c == 0.f ? b : 1.f) / SA);
+        e = by.next;
         float total = 0;
 #pragma unroll
         for (int i = 0; i < MINE; i++) {
@@ -335,7 +338,7 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) orthogonalize_small_kernel(c
                 for (int k = 0; k < 4; k++) {
                     uint32_t* xs = reinterpret_cast<uint32_t*>(X + slab_at(row0 + 8 * g, ch * 32 + 8 * k + 2 * q));
                     const float2 h = unpack(*xs), l = unpack(lo[i][g][k]);
-                    const float y0 = fmaf(w, h.x + l.x, f * x[g][k][0]), y1 = fmaf(w, h.y + l.y, f * x[g][k][1]);
+                    const float y0 = fmaf(by.w, h.x + l.x, by.g * x[g][k][0]), y1 = fmaf(by.w, h.y + l.y, by.g * x[g][k][1]);
                     x[g][k][0] = y0;
                     x[g][k][1] = y1;
                     if (!last) {

@@ -481,7 +481,8 @@ clblasStatus clblasB200I8gemm(
  *      G: FP32 / FP16 / BF16.  O: BF16 (the products take 11-bit operands: the result is good to about 1e-3 relative to
  *      its own norm).  beta == 0 never reads O.  A G that holds a NaN or an infinity gives NaN everywhere.  The iteration
  *      runs in FP16 with scale factors that leave room for singular values of X up to 16 and for |b| s^2 + |c| s^4 up to 255
- *      at singular values s; coefficients that drive X further overflow.
+ *      at singular values s; coefficients that drive X further overflow.  There is no lower end: a small X is held times a
+ *      power of two of its own, so a G whose norm is far below 1e-7 keeps the accuracy above.
  *      O may be G itself (BF16, same offset, pitch and stride); they may not overlap otherwise.  Matrices of G may overlap
  *      one another (strideG 0: one gradient), matrices of O may not.
  *      Workspace (from the library's pool): about 6 bytes per element of G and 4 per element of the smaller square; none up to
