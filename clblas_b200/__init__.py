@@ -197,6 +197,8 @@ def _load() -> ctypes.CDLL:
         f = getattr(lib, name)
         f.argtypes = [i, i, i, i, i, sz, sz, ft, vp, sz, sz, vp, sz, sz, vp, i, u, pvp, u, pvp, pvp]
         f.restype = i
+    lib.clblasB200BufferDevice.argtypes = [vp]
+    lib.clblasB200BufferDevice.restype = i
     lib.clblasB200QuantizeI8.argtypes = [i, i, sz, sz, i, vp, sz, sz, vp, sz, sz, vp, sz] + tail
     lib.clblasB200QuantizeI8.restype = i
     lib.clblasB200I8gemm.argtypes = [i, i, i, sz, sz, sz, ctypes.c_float, vp, sz, sz, vp, sz, vp, sz, sz, vp, sz,
@@ -218,7 +220,7 @@ EXPORTS = ["clblasSetup", "clblasTeardown", "clblasGetVersion", "clblasSgemm", "
     "clblasB200LastGemmVariant", "clblasB200WorkspaceAllocCount", "clblasB200NoAllocLimits", "clblasB200CommGetUniqueId",
     "clblasB200CommInitRank", "clblasB200CommInitAll", "clblasB200CommDestroy", "clblasB200CommInfo", "clblasB200PanelPlan",
     "clblasB200SgemmSharded", "clblasB200DgemmSharded", "clblasB200StrsmSharded", "clblasB200DtrsmSharded",
-    "clblasB200QuantizeI8", "clblasB200I8gemm", "clblasB200Orthogonalize"]
+    "clblasB200QuantizeI8", "clblasB200I8gemm", "clblasB200Orthogonalize", "clblasB200BufferDevice"]
 
 
 def _ptr(x) -> Optional[int]:
@@ -241,20 +243,30 @@ def _handle(x) -> Optional[int]:
     raise TypeError(f"not a CUDA stream or event: {x!r}")
 
 
-def _current_stream() -> int:
-    """Handle of torch's current stream on the current device (the raw query is some 3 us cheaper than building a Stream)."""
+def _result_device(x) -> Optional[int]:
+    """Ordinal of the device that holds a buffer; ``None`` where it is not known (the call is then refused, or it means the
+    current device)."""
+    if isinstance(x, int):
+        d = lib.clblasB200BufferDevice(x)
+        return d if d >= 0 else None
+    return getattr(getattr(x, "device", None), "index", None)
+
+
+def _current_stream(device: Optional[int] = None) -> int:
+    """Handle of torch's current stream on a device, ``None``: the current one (the raw query is some 3 us cheaper than building a
+    Stream)."""
     import torch
     try:
-        return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+        return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice() if device is None else device)
     except AttributeError:
-        return torch.cuda.current_stream().cuda_stream
+        return torch.cuda.current_stream(device).cuda_stream
 
 
-def _handle_array(items: Optional[Sequence], default_current_stream: bool = False):
+def _handle_array(items: Optional[Sequence], default_current_stream: bool = False, device: Optional[int] = None):
     if items is None:
         if not default_current_stream:
             return 0, None
-        items = [_current_stream()]
+        items = [_current_stream(device)]
     arr = (ctypes.c_void_p * max(len(items), 1))()
     for k, it in enumerate(items):
         arr[k] = _handle(it)
@@ -264,10 +276,11 @@ def _handle_array(items: Optional[Sequence], default_current_stream: bool = Fals
 _ONE_HANDLE = ctypes.c_void_p * 1
 
 
-def _queues_events(queues, wait, events):
+def _queues_events(queues, wait, events, device: Optional[int] = None):
+    """``device``: whose current stream is the default queue (``None``: the current device)."""
     if queues is None and wait is None and events is None:        # the common call: current stream, no events
-        return 1, _ONE_HANDLE(_current_stream()), 0, None, None
-    nq, q = _handle_array(queues, default_current_stream=True)
+        return 1, _ONE_HANDLE(_current_stream(device)), 0, None, None
+    nq, q = _handle_array(queues, default_current_stream=True, device=device)
     nw, w = _handle_array(wait)
     _, e = _handle_array(events)
     return nq, q, nw, w, e
@@ -310,8 +323,9 @@ def clblasDgemm(order, transA, transB, M, N, K, alpha, A, offA, lda, B, offB, ld
 def clblasB200QuantizeI8(order, side, M, N, typeX, X, offX, ldx, Q, offQ, ldq, scale, offScale,
                          queues=None, wait=None, events=None) -> int:
     """X (M x N, of ``clblasB200Float32`` / ``Float16`` / ``Bfloat16``) in signed 8-bit integers Q with one float32 scale per row
-    (``clblasLeft``: X ~ diag(scale) Q) or per column (``clblasRight``)."""
-    nq, q, nw, w, e = _queues_events(queues, wait, events)
+    (``clblasLeft``: X ~ diag(scale) Q) or per column (``clblasRight``).  ``queues`` defaults to torch's current stream on the device
+    that holds the result, here and in the two calls below."""
+    nq, q, nw, w, e = _queues_events(queues, wait, events, _result_device(Q) if queues is None else None)
     return lib.clblasB200QuantizeI8(order, side, M, N, typeX, _ptr(X), offX, ldx, _ptr(Q), offQ, ldq, _ptr(scale), offScale,
                                     nq, q, nw, w, e)
 
@@ -320,7 +334,7 @@ def clblasB200I8gemm(order, transA, transB, M, N, K, alpha, A, offA, lda, scaleA
                      beta, typeC, C, offC, ldc, queues=None, wait=None, events=None) -> int:
     """C <- alpha diag(scaleA) op(A) op(B) diag(scaleB) + beta C: A and B signed 8-bit integers, C of ``typeC``; the scales
     (float32, ``None``: ones) have M and N elements."""
-    nq, q, nw, w, e = _queues_events(queues, wait, events)
+    nq, q, nw, w, e = _queues_events(queues, wait, events, _result_device(C) if queues is None else None)
     return lib.clblasB200I8gemm(order, transA, transB, M, N, K, alpha, _ptr(A), offA, lda, _ptr(scaleA), offScaleA,
                                 _ptr(B), offB, ldb, _ptr(scaleB), offScaleB, beta, typeC, _ptr(C), offC, ldc, nq, q, nw, w, e)
 
@@ -334,7 +348,7 @@ def clblasB200Orthogonalize(order, M, N, batchCount, steps, coefficients, alpha,
         if len(flat) != 3 * steps:
             raise ValueError("coefficients: one (a, b, c) for each step")
         coefficients = (ctypes.c_float * len(flat))(*flat)
-    nq, q, nw, w, e = _queues_events(queues, wait, events)
+    nq, q, nw, w, e = _queues_events(queues, wait, events, _result_device(O) if queues is None else None)
     return lib.clblasB200Orthogonalize(order, M, N, batchCount, steps, coefficients, alpha, typeG, _ptr(G), offG, ldg, strideG,
                                        beta, _ptr(O), offO, ldo, strideO, nq, q, nw, w, e)
 

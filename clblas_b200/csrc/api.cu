@@ -1387,6 +1387,7 @@ clblasStatus clblasB200Orthogonalize(clblasOrder order, size_t M, size_t N, size
     return orthogonalize_entry(order, M, N, batchCount, steps, coefficients, alpha, (int)typeG, G, offG, ldg, strideG, beta, O, offO, ldo, strideO,
                                nq, queues, nev, wait, events);
 }
+int clblasB200BufferDevice(const clblasMem buffer) { return device_of(buffer); }
 int clblasB200SetGemmPath(int path) { return g_forced_path.exchange(path); }
 
 }  // extern "C"

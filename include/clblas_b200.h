@@ -520,6 +520,9 @@ const char* clblasB200LastGemmVariant(void);
  * (operand repacking, split-K and stream-K partial tiles, TRSM's inverted blocks ...).  A call across which the
  * number does not change allocated nothing. */
 unsigned long long clblasB200WorkspaceAllocCount(void);
+/* Ordinal of the device that holds a buffer, -1 when the driver does not know it: the device that the narrow-type routines
+ * run on when the buffer is their result, and whose queue they have to be given. */
+int clblasB200BufferDevice(const clblasMem buffer);
 /* The two size limits of clblasB200DtrsmNoAlloc as the built library has them (= the macros above). */
 void clblasB200NoAllocLimits(size_t* max_order, size_t* max_other);
 /* Forces a kernel family for GEMM calls of the whole process: 0 = automatic dispatch,
