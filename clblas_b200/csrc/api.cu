@@ -60,6 +60,13 @@ clblasStatus pick(ErrSet e, clblasStatus a, clblasStatus b, clblasStatus c)
     return e == SET_A ? a : (e == SET_B ? b : c);
 }
 
+// True when `lines` lines of `len` elements, ld >= len apart, behind `off` elements lie within `have` elements (lines, len >= 1).  By
+// divisions: a product of a huge leading dimension or offset would wrap round 2^64 and pass.
+bool extent_fits(size_t off, size_t lines, size_t len, size_t ld, size_t have)
+{
+    return off <= have && len <= have - off && (lines - 1) <= (have - off - len) / ld;
+}
+
 // checkMatrixSizes of the reference (src/library/blas/generic/common.c:585-686) for a non-packed
 // rows x cols matrix op(X).
 clblasStatus check_matrix_sizes(size_t tsize, clblasOrder order, clblasTranspose trans, size_t rows, size_t cols,
@@ -68,18 +75,11 @@ clblasStatus check_matrix_sizes(size_t tsize, clblasOrder order, clblasTranspose
     if (rows == 0 || cols == 0) return clblasInvalidDim;
     const bool tra = (order == clblasRowMajor && trans != clblasNoTrans) ||
                      (order == clblasColumnMajor && trans == clblasNoTrans);
-    size_t matr;
-    if (tra) {
-        if (ld < rows) return pick(e, clblasInvalidLeadDimA, clblasInvalidLeadDimB, clblasInvalidLeadDimC);
-        matr = ((cols - 1) * ld + rows) * tsize;
-    } else {
-        if (ld < cols) return pick(e, clblasInvalidLeadDimA, clblasInvalidLeadDimB, clblasInvalidLeadDimC);
-        matr = ((rows - 1) * ld + cols) * tsize;
-    }
+    const size_t lines = tra ? cols : rows, len = tra ? rows : cols;
+    if (ld < len) return pick(e, clblasInvalidLeadDimA, clblasInvalidLeadDimB, clblasInvalidLeadDimC);
     size_t avail = 0;
     if (!bytes_after(buf, &avail)) return pick(e, clblasInvalidMatA, clblasInvalidMatB, clblasInvalidMatC);
-    const size_t offb = off * tsize;
-    if (offb + matr > avail || offb + matr < offb)
+    if (!extent_fits(off, lines, len, ld, avail / tsize))
         return pick(e, clblasInsufficientMemMatA, clblasInsufficientMemMatB, clblasInsufficientMemMatC);
     return clblasSuccess;
 }
