@@ -292,10 +292,11 @@ cudaError_t i8gemm_typed(const I8GemmProblem& p, cudaStream_t s)
         return cudaGetLastError();
     }
     if (p.lines >= (1u << 31) || p.len >= (1u << 31)) return cudaErrorNotSupported;
-    auto usable = [](const void* q, size_t ld, bool kcontig) { return kcontig && aligned16(q) && ld % 16 == 0; };
-    const bool fixP = !usable(p.P, p.ldp, p.p_kcontig), fixQ = !usable(p.Q, p.ldq, p.q_kcontig);
+    // (One row has no pitch: any may be given, more than a tensor map takes too.)
+    auto usable = [](const void* q, size_t ld, bool kcontig, size_t rows) { return kcontig && aligned16(q) && (ld % 16 == 0 || rows == 1); };
+    const bool fixP = !usable(p.P, p.ldp, p.p_kcontig, p.lines), fixQ = !usable(p.Q, p.ldq, p.q_kcontig, p.len);
     const size_t kld = (p.K + 15) / 16 * 16;
-    Operand a{p.P, p.K, p.lines, p.ldp, 0}, b{p.Q, p.K, p.len, p.ldq, 0};
+    Operand a{p.P, p.K, p.lines, p.lines == 1 ? kld : p.ldp, 0}, b{p.Q, p.K, p.len, p.len == 1 ? kld : p.ldq, 0};
     unsigned char* ws = nullptr;
     cudaError_t e = cudaSuccess;
     if (fixP || fixQ) {

@@ -40,3 +40,21 @@ def test_offsets(buffers, off):
     assert cb.clblasB200QuantizeI8(0, 0, n, n, 0, f, 0, n, i, 0, n, f, off) == cb.clblasInsufficientMemVecX
     assert cb.clblasB200Orthogonalize(0, n, n, 1, 5, None, 1.0, 2, h, off, n, 0, 0.0, h, 0, n, 0) == cb.clblasInsufficientMemMatA
     assert cb.launch_count() == before
+
+
+@pytest.mark.parametrize("ld", [9, 1 << 45, 1 << 63, (1 << 64) - 1])
+def test_one_line_has_no_second(ld):
+    """A matrix of one line may have any leading dimension: no element lies behind it."""
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    x = torch.randn(9, generator=gen, device="cuda").bfloat16()
+    q, s, o, c = torch.zeros(9, dtype=torch.int8, device="cuda"), torch.zeros(1, device="cuda"), torch.zeros_like(x), torch.zeros(1, device="cuda")
+    cb.check(cb.clblasB200QuantizeI8(0, 0, 1, 9, 2, x, 0, ld, q, 0, ld, s, 0))
+    assert int(q.abs().max()) == 127
+    cb.check(cb.clblasB200I8gemm(0, 0, 1, 1, 1, 9, 1.0, q, 0, ld, None, 0, q, 0, ld, None, 0, 0.0, 0, c, 0, ld))
+    assert float(c) == float(q.double().square().sum())
+    cb.check(cb.clblasB200Orthogonalize(0, 1, 9, 1, 5, None, 1.0, 2, x, 0, ld, 0, 0.0, o, 0, ld, 0))
+    y = 1.0
+    for _ in range(5):
+        y *= 3.4445 - 4.775 * y ** 2 + 2.0315 * y ** 4
+    want = x.double() / x.double().norm() * y
+    assert float((o.double() - want).norm()) <= 5e-3 * abs(y) and cb.lib.clblasB200DeviceFault() == 0
