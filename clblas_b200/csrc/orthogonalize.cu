@@ -423,7 +423,7 @@ cudaError_t orthogonalize_typed(const OrthProblem& p, cudaStream_t s)
     if (orthogonalize_small_applies(p)) return orthogonalize_small<T>(p, s);
     const bool flip = p.lines > p.len;
     const size_t n = flip ? p.len : p.lines, m = flip ? p.lines : p.len, batch = p.batch;
-    if (m >= (1u << 31) || batch >= 65536) return cudaErrorNotSupported;
+    if (m >= (1u << 31)) return cudaErrorNotSupported;
     auto up = [](size_t v, size_t q) { return (v + q - 1) / q * q; };
     const size_t ldx = up(m, 8), ldn = up(n, 8), xs = n * ldx, as = n * ldn;
     const int pitch = p.steps + 1;
@@ -491,11 +491,22 @@ cudaError_t orthogonalize_typed(const OrthProblem& p, cudaStream_t s)
 
 cudaError_t orthogonalize(const OrthProblem& p, cudaStream_t s)
 {
-    switch (p.type) {
-        case clblasB200Float32: return orthogonalize_typed<float>(p, s);
-        case clblasB200Float16: return orthogonalize_typed<__half>(p, s);
-        default: return orthogonalize_typed<__nv_bfloat16>(p, s);
+    // A grid has 65535 blocks along y, the matrices of a batch: larger batches in parts, which share a workspace in turn.
+    constexpr size_t MOST = 32768;
+    for (size_t i = 0; i < p.batch; i += MOST) {
+        OrthProblem part = p;
+        part.batch = std::min(MOST, p.batch - i);
+        part.offG += i * p.strideG;
+        part.offO += i * p.strideO;
+        cudaError_t e;
+        switch (p.type) {
+            case clblasB200Float32: e = orthogonalize_typed<float>(part, s); break;
+            case clblasB200Float16: e = orthogonalize_typed<__half>(part, s); break;
+            default: e = orthogonalize_typed<__nv_bfloat16>(part, s);
+        }
+        if (e != cudaSuccess) return e;
     }
+    return cudaSuccess;
 }
 
 unsigned orthogonalize_fault_flag() { return read_wait_timeout_flag() | orthogonalize_small_fault_flag(); }

@@ -463,7 +463,6 @@ cudaError_t orthogonalize_small(const OrthProblem& p, cudaStream_t s)
         k.coeffs[3 * i + 1] = p.coeffs ? p.coeffs[3 * i + 1] : -4.7750f;
         k.coeffs[3 * i + 2] = p.coeffs ? p.coeffs[3 * i + 2] : 2.0315f;
     }
-    if (p.batch >= (1u << 27)) return cudaErrorNotSupported;
     switch (ranks) {
         case 1: return launch_small<T, 1>(k, p.batch, s);
         case 2: return launch_small<T, 2>(k, p.batch, s);

@@ -451,7 +451,8 @@ typedef enum clblasB200Type_ { clblasB200Float32 = 0, clblasB200Float16 = 1, clb
  *          scale = max|x| / 127,   q = rint(x * (127 / max|x|)),   each operation one IEEE FP32 operation, ties to even.
  *      A row (column) of magnitudes below 2^-100 counts as zero: scale 0, q 0.  One that holds a NaN or an infinity gets
  *      scale NaN and q 0, so that every product with it is NaN.
- *      Checks: X (A's status codes), Q (B's), scale (clblasInvalidVecX, clblasInsufficientMemVecX). */
+ *      Checks: X (A's status codes), Q (B's), scale (clblasInvalidVecX, clblasInsufficientMemVecX).  2^31 rows (columns of a
+ *      column-major X) and more, one scale for each, are clblasNotImplemented. */
 clblasStatus clblasB200QuantizeI8(
     clblasOrder order, clblasSide side, size_t M, size_t N,
     clblasB200Type typeX, const clblasMem X, size_t offX, size_t ldx,
@@ -464,7 +465,8 @@ clblasStatus clblasB200QuantizeI8(
  *      scaleA: M and scaleB: N FP32 values (NULL: ones).  op(A)*op(B) is exact (32-bit integers; K <= 131071, else
  *      clblasInvalidDim); the scaling is FP32 and C is rounded once.  beta == 0 never reads C; alpha == 0 or K == 0
  *      never reads A, B or the scales.
- *      Checks: those of clblasSgemm in its order, then the scales (VecX for scaleA, VecY for scaleB). */
+ *      Checks: those of clblasSgemm in its order, then the scales (VecX for scaleA, VecY for scaleB).  M or N of 2^31 and more
+ *      is clblasNotImplemented. */
 clblasStatus clblasB200I8gemm(
     clblasOrder order, clblasTranspose transA, clblasTranspose transB, size_t M, size_t N, size_t K, float alpha,
     const clblasMem A, size_t offA, size_t lda, const clblasMem scaleA, size_t offScaleA,
@@ -487,7 +489,8 @@ clblasStatus clblasB200I8gemm(
  *      one another (strideG 0: one gradient), matrices of O may not.
  *      Workspace (from the library's pool): about 6 bytes per element of G and 4 per element of the smaller square; none up to
  *      128 x 2048.
- *      Checks: G (A's status codes), O (C's; clblasInvalidLeadDimC also for a stride that makes its matrices overlap). */
+ *      Checks: G (A's status codes), O (C's; clblasInvalidLeadDimC also for a stride that makes its matrices overlap).
+ *      A side of 2^31 and more is clblasNotImplemented; batchCount is as large as the buffers. */
 clblasStatus clblasB200Orthogonalize(
     clblasOrder order, size_t M, size_t N, size_t batchCount, unsigned steps, const float* coefficients, float alpha,
     clblasB200Type typeG, const clblasMem G, size_t offG, size_t ldg, size_t strideG,
