@@ -5,8 +5,8 @@
 //
 // On the smaller side n of the matrix (n <= m) a step is three products: the Gram matrix (symmetric, n^2 m operations), its
 // square (symmetric, n^3) and the update (2 n^2 m).  All run on the FP16 tensor-core tiles of narrow_mma.cuh, the symmetric ones on
-// the tiles of one triangle, each result stored at both places.  (Matrices up to 128 x 2048 take one kernel instead of the
-// chain: orthogonalize_small.cu.)
+// the tiles of one triangle, each result stored at both places.  (Matrices up to 128 x 1024, and up to 128 x 2048 where
+// there are at most 15, take one kernel instead of the chain: orthogonalize_small.cu.)
 //
 // Measured, five steps: 4096 x 16384 BF16 3.65 ms alone, 4.2 ms back to back under the power cap (Gram 205 us, square 61, update 410: the
 // tiles without their epilogues 329, the rest is the 8 bytes an element that X costs to read and write); twelve 768 x 768 FP32 265 us

@@ -1,5 +1,5 @@
-// Newton-Schulz orthogonalisation of matrices whose smaller side is at most 128 and whose larger is at most 2048, all steps in one
-// kernel: a cluster of up to 8 CTAs holds a matrix on chip.  (The iteration, its roundings and its scales: orthogonalize.cu.)
+// Newton-Schulz orthogonalisation of matrices whose smaller side is at most 128 and whose larger is at most 1024 (2048 where there are at
+// most 15: orthogonalize_small_applies), all steps in one kernel: a cluster of up to 8 CTAs holds a matrix on chip.  (The iteration, its roundings and its scales: orthogonalize.cu.)
 //
 // CTA r of a cluster keeps W columns of X (n <= 128 rows, padded to 128): hi in shared memory, as 64-column slabs of SWIZZLE_128B rows,
 // lo in registers, always in the same fragments of the same threads.  One copy of hi serves both products: as
