@@ -36,6 +36,7 @@ template <> __device__ __forceinline__ float2 unpack16<__nv_bfloat16>(uint32_t h
 template <typename T>
 struct EpiScaled {
     static constexpr bool kHeavy = sizeof(T) == 4;
+    static constexpr bool kTriangle = false;
     struct State { float factor[4]; };
     template <int G> struct Pre { Bits16<G> c; };
     // Scales of the rows u and the columns v; nullptr: ones.  Read by ordinary loads after pdl_wait() and not as constants (__ldg): the

@@ -184,12 +184,11 @@ __device__ __forceinline__ float acc_value(uint32_t v) { return KIND == KIND_I8 
 struct Shape {
     unsigned U, V, K, batch;
     unsigned tilesU, tilesV, tiles;           // tiles: per batch entry (of the lower triangle when tri)
-    int tri;                                  // 1: U == V, symmetric: tiles that touch the lower triangle only (in blocks of 128 x 128)
-    unsigned per;                             // tri: columns of tiles per row of tiles (tile height / tile width, 1 or 2)
+    int tri;                                  // 1: U == V, symmetric: square tiles, those that touch the lower triangle only
 };
 
-// What becomes of a chunk: its 128 x 128 block lies below the diagonal (stored at both places), on it, or above (a tile that
-// straddles the diagonal; not stored).
+// What becomes of a chunk: its 128 x 128 block lies below the diagonal (stored at both places), on it, or above (in a 256 x 256 tile on
+// the diagonal; not stored).
 enum Part { PART_PLAIN = 0, PART_BELOW = 1, PART_ABOVE = -1 };
 __device__ __forceinline__ int part_of(const Shape& s, unsigned u0, unsigned v0)
 {
@@ -203,13 +202,12 @@ __device__ __forceinline__ int part_of(const Shape& s, unsigned u0, unsigned v0)
 constexpr unsigned GROUP = 8;
 __host__ __device__ inline void tile_coords(const Shape& s, unsigned t, unsigned& tu, unsigned& tv)
 {
-    if (s.tri) {                              // row r has per * (r + 1) tiles
-        const unsigned p = t / s.per;
-        unsigned r = (unsigned)((sqrtf(8.0f * (float)p + 1.0f) - 1.0f) * 0.5f);
-        while (r * (r + 1) / 2 > p) r--;
-        while ((r + 1) * (r + 2) / 2 <= p) r++;
+    if (s.tri) {                              // row r has r + 1 tiles
+        unsigned r = (unsigned)((sqrtf(8.0f * (float)t + 1.0f) - 1.0f) * 0.5f);
+        while (r * (r + 1) / 2 > t) r--;
+        while ((r + 1) * (r + 2) / 2 <= t) r++;
         tu = r;
-        tv = t - s.per * (r * (r + 1) / 2);
+        tv = t - r * (r + 1) / 2;
         return;
     }
     const unsigned per_group = GROUP * s.tilesV, g = t / per_group, first = g * GROUP, left = s.tilesU - first;
@@ -222,6 +220,7 @@ __host__ __device__ inline void tile_coords(const Shape& s, unsigned t, unsigned
 // Epilogue.  A warp finishes chunks of 32 rows x 8 G columns, held as fragments x[g][k][e]: row 8 g + lane / 4, column
 // 8 k + 2 (lane % 4) + e.  What a functor has:
 //   kHeavy        reads as much as it writes (for choose_plan)
+//   kTriangle     of symmetric products (Shape::tri)
 //   begin()       per thread and tile; u0, v0: where the warp's first chunk begins (of all its tiles one warp has both 0)
 //   Pre, fetch()  what a chunk needs besides the accumulators, requested one chunk ahead
 //   chunk()       computes and stores (where: part_of()); requests the next chunk's (at column v_next, ~0u: none) as soon as its own is used
@@ -758,8 +757,7 @@ inline void set_tiles(Shape& s, unsigned bu, unsigned bv)
 {
     s.tilesU = (s.U + bu - 1) / bu;
     s.tilesV = (s.V + bv - 1) / bv;
-    s.per = bu / bv;
-    s.tiles = s.tri ? s.per * (s.tilesU * (s.tilesU + 1) / 2) : s.tilesU * s.tilesV;
+    s.tiles = s.tri ? s.tilesU * (s.tilesU + 1) / 2 : s.tilesU * s.tilesV;
 }
 
 template <typename Kernel, typename Epi>
@@ -844,14 +842,15 @@ inline Plan choose_plan(unsigned U, unsigned V, unsigned K, unsigned batch, int 
     const double sms = sm_count();
     auto tiles = [&](unsigned bu, unsigned bv) {
         const double tu = (U + bu - 1) / bu, tv = (V + bv - 1) / bv;
-        return batch * (tri ? (double)(bu / bv) * tu * (tu + 1) / 2 : tu * tv);
+        return batch * (tri ? tu * (tu + 1) / 2 : tu * tv);
     };
     Plan best{};
     double least = 1e30;
     auto consider = [&](Plan plan, double us) { if (us < least) { least = us; best = plan; } };
     const double pairs = std::floor(sms / 2), t256 = tiles(256, 256), t128 = tiles(128, 128), e256 = heavy ? 8.5 : 5.0, e128 = heavy ? 7.0 : 5.0;
     consider({256, 0}, 5 + nk * (0.30 + 0.07 * std::fmin(1.0, t256 / pairs)) + e256 + (std::ceil(t256 / pairs) - 1) * std::fmax(nk * (heavy ? 0.45 : 0.36), e256));
-    consider({128, 0}, 5 + nk * 0.30 + 0.7 * e128 + (std::ceil(tiles(256, 128) / pairs) - 1) * std::fmax(nk * 0.37, e128));
+    // (For triangles never the shortest: up to one round, 74 tiles, 128 x 128 tiles take 0.5 less, beyond it 256 x 256 ones half the rounds.)
+    if (!tri) consider({128, 0}, 5 + nk * 0.30 + 0.7 * e128 + (std::ceil(tiles(256, 128) / pairs) - 1) * std::fmax(nk * 0.37, e128));
     if (kind == KIND_I8)
         consider({192, 0}, 5 + nk * 0.33 + 0.75 * e256 + 0.5 + (std::ceil(tiles(256, 192) / pairs) - 1) * std::fmax(nk * (heavy ? 0.40 : 0.33), 0.75 * e256 + 0.5));
     const double finish[3] = {heavy ? 6.3 : 5.0, heavy ? 5.6 : 4.6, heavy ? 4.5 : 4.2};
@@ -877,7 +876,8 @@ cudaError_t run_planned(const Operand& p, const Operand& q, const Shape& s, cons
 {
     const Plan plan = choose_plan(s.U, s.V, s.K, s.batch, s.tri, KIND, Epi::kHeavy);
     if (plan.pairs == 256) return run_persistent<KIND, 256, QMN, Epi>(p, q, s, epi, st);
-    if (plan.pairs == 128) return run_persistent<KIND, 128, QMN, Epi>(p, q, s, epi, st);
+    if constexpr (!Epi::kTriangle)
+        if (plan.pairs == 128) return run_persistent<KIND, 128, QMN, Epi>(p, q, s, epi, st);
     if constexpr (KIND == KIND_I8)
         if (plan.pairs == 192) return run_persistent<KIND, 192, QMN, Epi>(p, q, s, epi, st);
     return run_split_by<KIND, 128, QMN, Epi>(plan.split, p, q, s, epi, st);

@@ -204,6 +204,7 @@ __device__ __forceinline__ const uint16_t* bits(const __half* p) { return reinte
 
 struct EpiGram {                                           // A <- X X' - t I
     static constexpr bool kHeavy = false;
+    static constexpr bool kTriangle = true;
     struct State { float t; };
     template <int G> struct Pre {};
     __half* A; size_t ld, stride;
@@ -247,6 +248,7 @@ struct EpiGram {                                           // A <- X X' - t I
 
 struct EpiSquare {                                         // P <- (b + 2 c t) A + c A^2, times 2^p
     static constexpr bool kHeavy = false;
+    static constexpr bool kTriangle = true;
     struct State { float b, f; };
     template <int G> struct Pre { Bits16<G> a; };
     const __half* A; __half* P; size_t ld, stride;
@@ -316,6 +318,7 @@ struct UpdateTerm {
 
 struct EpiUpdate {
     static constexpr bool kHeavy = true;
+    static constexpr bool kTriangle = false;
     struct State { UpdateTerm::Factors by; float sum; };
     template <int G> using Pre = UpdateTerm::Pre<G>;
     UpdateTerm t;
@@ -367,6 +370,7 @@ struct EpiUpdate {
 
 struct EpiOut {                                            // O <- alpha X + beta O
     static constexpr bool kHeavy = true;
+    static constexpr bool kTriangle = false;
     struct State { UpdateTerm::Factors by; };
     template <int G> struct Pre { UpdateTerm::Pre<G> x; Bits16<G> o; };
     UpdateTerm t;
