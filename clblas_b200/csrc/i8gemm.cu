@@ -10,6 +10,8 @@
 // aligned, is transposed / copied once into a workspace.
 #include "narrow_mma.cuh"
 
+#include <cstdio>
+
 namespace cb200 {
 
 namespace {
@@ -317,6 +319,11 @@ cudaError_t i8gemm_typed(const I8GemmProblem& p, cudaStream_t s)
         if (e == cudaSuccess) count_launch();
     }
     if (e == cudaSuccess) e = multiply<T>(a, b, p.s_lines, p.s_len, p.alpha, p.beta, C, p.ldc, s);
+    if (e == cudaSuccess) {
+        char name[64];
+        std::snprintf(name, sizeof(name), "i8gemm_tcgen05<%s>", last_plan());
+        set_last_variant(name);
+    }
     if (ws) {
         const cudaError_t e2 = ws_free(ws, s);
         if (e == cudaSuccess) e = e2;
@@ -329,7 +336,6 @@ cudaError_t i8gemm_typed(const I8GemmProblem& p, cudaStream_t s)
 cudaError_t i8gemm(const I8GemmProblem& p, cudaStream_t s)
 {
     set_last_kernel("i8gemm_tcgen05");
-    set_last_variant("i8gemm_tcgen05");
     switch (p.type) {
         case clblasB200Float32: return i8gemm_typed<float>(p, s);
         case clblasB200Float16: return i8gemm_typed<__half>(p, s);

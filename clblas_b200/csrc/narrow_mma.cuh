@@ -785,6 +785,20 @@ cudaError_t launch(Kernel kernel, unsigned grid, unsigned cluster, int smem, cud
     return e;
 }
 
+// Name of the plan of the calling thread's last product (for clblasB200LastGemmVariant).
+inline const char*& last_plan()
+{
+    static thread_local const char* name = "";
+    return name;
+}
+constexpr const char* plan_name(int bn, int split)        // split 0: pairs
+{
+    if (split == 0) return bn == 256 ? "pairs256" : bn == 192 ? "pairs192" : "pairs128";
+    if (bn == 32) return split == 1 ? "split32x1" : split == 2 ? "split32x2" : split == 4 ? "split32x4" : "split32x8";
+    if (bn == 64) return split == 1 ? "split64x1" : split == 2 ? "split64x2" : split == 4 ? "split64x4" : "split64x8";
+    return split == 1 ? "split128x1" : split == 2 ? "split128x2" : "split128x4";
+}
+
 template <int KIND, int BN, bool QMN, class Epi>
 cudaError_t run_persistent(const Operand& p, const Operand& q, Shape s, const Epi& epi, cudaStream_t st)
 {
@@ -799,6 +813,7 @@ cudaError_t run_persistent(const Operand& p, const Operand& q, Shape s, const Ep
         !make_map(&mq, KIND, q.base, q.inner, q.rows, s.batch, q.ld, q.stride, QMN ? slab_k(KIND) : BN / CG))
         return cudaErrorNotSupported;
     set_tiles(s, BM * CG, BN);
+    last_plan() = plan_name(BN, 0);
     const unsigned slots = (unsigned)sm_count() / CG, work = s.tiles * s.batch;
     return launch(kernel, CG * (work < slots ? work : slots), CG, smem, st, mp, mq, s, epi);
 }
@@ -816,6 +831,7 @@ cudaError_t run_split(const Operand& p, const Operand& q, Shape s, const Epi& ep
         !make_map(&mq, KIND, q.base, q.inner, q.rows, s.batch, q.ld, q.stride, QMN ? slab_k(KIND) : BN))
         return cudaErrorNotSupported;
     set_tiles(s, BM, BN);
+    last_plan() = plan_name(BN, S);
     return launch(kernel, s.tiles * s.batch * S, S, smem, st, mp, mq, s, epi);
 }
 

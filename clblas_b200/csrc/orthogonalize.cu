@@ -29,6 +29,7 @@
 #include "orthogonalize.cuh"
 
 #include <algorithm>
+#include <cstdio>
 #include <type_traits>
 
 namespace cb200 {
@@ -463,6 +464,7 @@ cudaError_t orthogonalize_typed(const OrthProblem& p, cudaStream_t s)
         if (vec) e = flip ? prepare(std::true_type{}, std::true_type{}) : prepare(std::true_type{}, std::false_type{});
         else     e = flip ? prepare(std::false_type{}, std::true_type{}) : prepare(std::false_type{}, std::false_type{});
     }
+    const char* plans[2] = {"", "none"};                   // of the last step's products
     for (int k = 0; k < p.steps && e == cudaSuccess; k++) {
         const float a = p.coeffs ? p.coeffs[3 * k] : 3.4445f, b = p.coeffs ? p.coeffs[3 * k + 1] : -4.7750f, c = p.coeffs ? p.coeffs[3 * k + 2] : 2.0315f;
         const Sizes sizes{sums + k, exps + k, factors + k, pitch, (float)n, a, b, c, k + 1 == p.steps, p.alpha / SX};
@@ -471,9 +473,11 @@ cudaError_t orthogonalize_typed(const OrthProblem& p, cudaStream_t s)
         Shape sq = {};
         sq.U = sq.V = (unsigned)n; sq.K = (unsigned)m; sq.batch = (unsigned)batch; sq.tri = 1;
         e = run_planned<KIND_F16, false>(ox, ox, sq, EpiGram{A, ldn, as, sizes}, s);
+        plans[0] = last_plan();
         if (e == cudaSuccess && c != 0.f) {
             sq.K = (unsigned)n;
             e = run_planned<KIND_F16, false>(oa, oa, sq, EpiSquare{A, P, ldn, as, factors + k, pitch}, s);
+            plans[1] = last_plan();
         }
         if (e != cudaSuccess) break;
         Shape up_ = {};
@@ -486,6 +490,11 @@ cudaError_t orthogonalize_typed(const OrthProblem& p, cudaStream_t s)
             const int align = line_alignment(O, p.ldo, batch > 1 ? p.strideO : 0);
             e = run_planned<KIND_F16, true>(c != 0.f ? op : oa, ox, up_, EpiOut{t, O, p.ldo, p.strideO, p.beta, flip, align}, s);
         }
+    }
+    if (e == cudaSuccess) {
+        char name[96];
+        std::snprintf(name, sizeof(name), "orthogonalize<%s,%s,%s>", plans[0], plans[1], last_plan());
+        set_last_variant(name);
     }
     const cudaError_t e2 = ws_free(ws, s);
     return e == cudaSuccess ? e2 : e;

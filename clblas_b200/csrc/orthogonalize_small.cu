@@ -463,6 +463,7 @@ cudaError_t orthogonalize_small(const OrthProblem& p, cudaStream_t s)
         k.coeffs[3 * i + 1] = p.coeffs ? p.coeffs[3 * i + 1] : -4.7750f;
         k.coeffs[3 * i + 2] = p.coeffs ? p.coeffs[3 * i + 2] : 2.0315f;
     }
+    set_last_variant(ranks == 1 ? "orthogonalize_small<1>" : ranks == 2 ? "orthogonalize_small<2>" : ranks == 4 ? "orthogonalize_small<4>" : "orthogonalize_small<8>");
     switch (ranks) {
         case 1: return launch_small<T, 1>(k, p.batch, s);
         case 2: return launch_small<T, 2>(k, p.batch, s);

@@ -517,7 +517,9 @@ double clblasB200ProbePeak(int kind, double seconds);
 const char* clblasB200LastGemmKernel(void);
 /* The instantiation and mode behind that name, e.g. "dgemm_mma_tma<T,N,128>+streamk_tail",
  * "sgemm_ffma_tma<N,N,64,3,2>+splitk2", "sgemm_nt_16x8+tri": lets a test assert which variant it exercised.
- * Thread-local storage, overwritten by the thread's next GEMM; never NULL. */
+ * Of the narrow-type routines: "i8gemm_tcgen05<pairs256>" (tiles on pairs of CTAs), "i8gemm_tcgen05<split32x4>" (tiles of 32
+ * columns, k over 4 CTAs), "orthogonalize<Gram product,square,update>" with a plan for each, "orthogonalize_small<CTAs>".
+ * Thread-local storage, overwritten by the thread's next GEMM or orthogonalisation; never NULL. */
 const char* clblasB200LastGemmVariant(void);
 /* Number of workspace allocations the level-3 routines of this library have made in the calling process so far
  * (operand repacking, split-K and stream-K partial tiles, TRSM's inverted blocks ...).  A call across which the
