@@ -18,10 +18,22 @@ def exponent_of(v):
     return math.frexp(v)[1]
 
 
-def orth_emulated(g, coefficients, shift=True, low=True, gram=half, scaled=True):
+def product(a, b):
+    return a @ b
+
+
+def truncating_product(a, b):
+    """A sum in FP32 that is cut off after every 16 terms: no accumulator of a k = 16 instruction is worse."""
+    acc = torch.zeros(a.shape[0], b.shape[1], dtype=torch.float64, device=a.device)
+    for k in range(0, a.shape[1], 16):
+        acc = ((acc + a[:, k:k + 16] @ b[k:k + 16]).view(torch.int64) & ~((1 << 29) - 1)).view(torch.float64)
+    return acc
+
+
+def orth_emulated(g, coefficients, shift=True, low=True, gram=half, scaled=True, mul=product):
     """NS(G), rows x cols, as the operator rounds it: X = hi + lo in two FP16 numbers times 2^e, the products take hi, the Gram matrix
     minus its mean diagonal and the polynomial are FP16; sums are exact here.  The switches leave out what the design rests on
-    (the shift, the low half, FP16 for the Gram matrix, the power of two), for tests of the tests."""
+    (the shift, the low half, FP16 for the Gram matrix, the power of two), for tests of the tests; mul: how products are summed."""
     g = g.double()
     flip = g.shape[0] > g.shape[1]
     if flip:
@@ -37,14 +49,14 @@ def orth_emulated(g, coefficients, shift=True, low=True, gram=half, scaled=True)
         q2 = float((y / SX).square().sum())
         mean = q2 / n
         t = mean if shift and mean * 4.0 ** -e >= 0.2 else 0.0
-        A = gram(hi @ hi.t() * (SA / SX ** 2) - SA * t * eye)
+        A = gram(mul(hi, hi.t()) * (SA / SX ** 2) - SA * t * eye)
         grown = abs(b) * q2 + abs(c) * q2 * q2 * 4.0 ** -e
         p = max(0, 2 * e - exponent_of(grown)) if scaled and grown > 0 else 0
         bk, ck = b * 4.0 ** -e, c * 16.0 ** -e
-        P = half(2.0 ** p * ((bk + 2 * ck * t) * A + (ck / SA) * (A @ A))) * 2.0 ** -p if c else bk * A
+        P = half(2.0 ** p * ((bk + 2 * ck * t) * A + (ck / SA) * mul(A, A))) * 2.0 ** -p if c else bk * A
         bound = math.sqrt(q2) * (abs(a) + grown * 4.0 ** -e)
         after = max(0, e - exponent_of(bound)) if scaled and bound > 0 else e
-        y = ((a + t * (bk + ck * t)) * (hi + lo) + P @ hi / SA) * 2.0 ** (after - e)
+        y = ((a + t * (bk + ck * t)) * (hi + lo) + mul(P, hi) / SA) * 2.0 ** (after - e)
         e = after
     x = y / SX * 2.0 ** -e
     return x.t() if flip else x
