@@ -22,7 +22,9 @@
 //     halves the error of the result (normal 768 x 768: 1.5e-3 without, 7e-4 with t; the final rounding to BF16 is 1.7e-3).
 //   * t comes from the sum of the squares of X, gathered in 64-bit integers (units of 2^-24), so the order of the atomic additions does
 //     not change it.  Any t gives the same polynomial; it only has to be near.
-//   * Accumulators and everything between accumulator and store are FP32.  X is held times 2^12, A and P times 2^8, so that the
+//   * Accumulators and everything between accumulator and store are FP32.  The tensor core cuts its sums off instead of rounding them, so a
+//     long one falls behind, by about 2^-25 for every 16 terms (8 x 2^20: 1.5e-3 of the result, 8 x 2^24: 2.3 %).  Beyond SEGMENT elements the Gram
+//     product is therefore taken in segments, which are added up in ordinary FP32 (8 x 2^24: 1.9e-4).  X is held times 2^12, A and P times 2^8, so that the
 //     entries of large matrices (about 1/sqrt(m)) stay far above FP16's smallest numbers, and times a power of two for each matrix where
 //     the whole matrix is small (orthogonalize.cuh).  768 x 768, |G|_F = 1e-15: 32 % off without that power, 3.4e-4 with it.
 // The result is good to about 1e-3 and is therefore given in BF16 only.
@@ -203,6 +205,56 @@ struct Sizes {
 __device__ __forceinline__ uint16_t* bits(__half* p) { return reinterpret_cast<uint16_t*>(p); }
 __device__ __forceinline__ const uint16_t* bits(const __half* p) { return reinterpret_cast<const uint16_t*>(p); }
 
+// The product of one segment of X: S <- X X' or S + X X', on the tiles of the triangle.
+struct EpiGramPart {
+    static constexpr bool kHeavy = false;
+    static constexpr bool kTriangle = true;
+    struct State {};
+    template <int G> struct Pre {};
+    float* S; size_t ld, stride;
+    bool first;
+    // x += what S holds at its place (the same in all kernels: each element is read and written by one thread)
+    template <int G>
+    __device__ static void add(const float* S, size_t ld, const Shape& s, unsigned u0, unsigned v0, float (&x)[4][G][2])
+    {
+        const int lane = threadIdx.x & 31;
+        float2 old[4][G];
+#pragma unroll
+        for (int g = 0; g < 4; g++)
+#pragma unroll
+            for (int k = 0; k < G; k++) {
+                const unsigned u = u0 + 8 * g + lane / 4, v = v0 + 8 * k + 2 * (lane & 3);
+                old[g][k] = u < s.U && v < s.V ? *reinterpret_cast<const float2*>(S + (size_t)u * ld + v) : make_float2(0.f, 0.f);
+            }
+#pragma unroll
+        for (int g = 0; g < 4; g++)
+#pragma unroll
+            for (int k = 0; k < G; k++) {
+                x[g][k][0] += old[g][k].x;
+                x[g][k][1] += old[g][k].y;
+            }
+    }
+    __device__ void begin(State&, const Shape&, unsigned, unsigned, unsigned) const {}
+    template <int G> __device__ void fetch(Pre<G>&, const Shape&, unsigned, unsigned, unsigned) const {}
+    template <int G>
+    __device__ void chunk(State&, Pre<G>&, const Shape& s, unsigned z, unsigned u0, unsigned v0, unsigned, int where, float (&x)[4][G][2]) const
+    {
+        if (where == PART_ABOVE) return;
+        float* to = S + z * stride;
+        if (!first) add<G>(to, ld, s, u0, v0, x);
+        const int lane = threadIdx.x & 31;
+#pragma unroll
+        for (int g = 0; g < 4; g++)
+#pragma unroll
+            for (int k = 0; k < G; k++) {
+                const unsigned u = u0 + 8 * g + lane / 4, v = v0 + 8 * k + 2 * (lane & 3);      // the pitch is even: v + 1 is padding at most
+                if (u < s.U && v < s.V) *reinterpret_cast<float2*>(to + (size_t)u * ld + v) = make_float2(x[g][k][0], x[g][k][1]);
+            }
+    }
+    __device__ void end(State&, unsigned, unsigned) const {}
+};
+
+template <bool JOIN>                                       // JOIN: of the last segment, S holds the sum of the others
 struct EpiGram {                                           // A <- X X' - t I
     static constexpr bool kHeavy = false;
     static constexpr bool kTriangle = true;
@@ -210,6 +262,7 @@ struct EpiGram {                                           // A <- X X' - t I
     template <int G> struct Pre {};
     __half* A; size_t ld, stride;
     Sizes sizes;
+    const float* S;
     __device__ void begin(State& st, const Shape&, unsigned z, unsigned u0, unsigned v0) const
     {
         const size_t at = (size_t)z * sizes.pitch;         // read past L1: a neighbour is written meanwhile
@@ -228,6 +281,7 @@ struct EpiGram {                                           // A <- X X' - t I
     template <int G>
     __device__ void chunk(State& st, Pre<G>&, const Shape& s, unsigned z, unsigned u0, unsigned v0, unsigned, int where, float (&x)[4][G][2]) const
     {
+        if (JOIN && where != PART_ABOVE) EpiGramPart::add<G>(S + z * stride, ld, s, u0, v0, x);
         const int lane = threadIdx.x & 31;
         const int off = (int)(u0 + lane / 4) - (int)(v0 + 2 * (lane & 3));      // row - column of x[0][0][0]
         Bits16<G> o;
@@ -420,6 +474,9 @@ struct EpiOut {                                            // O <- alpha X + bet
     __device__ void end(State&, unsigned, unsigned) const {}
 };
 
+// Longest sum of a Gram product: an error of up to 2.5e-4 on its diagonal, half of what rounding A to FP16 costs.
+constexpr size_t SEGMENT = 1 << 17;
+
 // ---- the chain ----------------------------------------------------------------------------------------------------------
 
 template <typename T>
@@ -435,10 +492,11 @@ cudaError_t orthogonalize_typed(const OrthProblem& p, cudaStream_t s)
     // Blocks of the norm: about 8 pieces a thread, at most two blocks per SM over the batch.
     const size_t blocks = (p.lines * ((p.len + 7) / 8) + 2047) / 2048, most = std::max<size_t>(1, 2 * (size_t)sm_count() / batch);
     const size_t parts = std::min(blocks, most);
-    // workspace: hi (two of them, read and written in turn), lo, A, P, sums of squares, exponents, factors, partial norms
-    const size_t x_bytes = up(batch * xs * 2, 256), a_bytes = up(batch * as * 2, 256), sum_bytes = up(batch * pitch * 8, 256), exp_bytes = up(batch * pitch * 4, 256), factor_bytes = up(batch * pitch * 16, 256);
+    // workspace: hi (two of them, read and written in turn), lo, A, P, sums of squares, exponents, factors, partial norms, sums of segments
+    const size_t x_bytes = up(batch * xs * 2, 256), a_bytes = up(batch * as * 2, 256), sum_bytes = up(batch * pitch * 8, 256), exp_bytes = up(batch * pitch * 4, 256), factor_bytes = up(batch * pitch * 16, 256),
+                 part_bytes = up(batch * parts * 8, 256), join_bytes = m > SEGMENT ? batch * as * 4 : 0;
     unsigned char* ws = nullptr;
-    cudaError_t e = ws_alloc(reinterpret_cast<void**>(&ws), 3 * x_bytes + 2 * a_bytes + sum_bytes + exp_bytes + factor_bytes + batch * parts * 8, s);
+    cudaError_t e = ws_alloc(reinterpret_cast<void**>(&ws), 3 * x_bytes + 2 * a_bytes + sum_bytes + exp_bytes + factor_bytes + part_bytes + join_bytes, s);
     if (e != cudaSuccess) return e;
     __half* hi[2] = {reinterpret_cast<__half*>(ws), reinterpret_cast<__half*>(ws + x_bytes)};
     __half* lo = reinterpret_cast<__half*>(ws + 2 * x_bytes);
@@ -448,6 +506,7 @@ cudaError_t orthogonalize_typed(const OrthProblem& p, cudaStream_t s)
     int* exps = reinterpret_cast<int*>(ws + 3 * x_bytes + 2 * a_bytes + sum_bytes);
     float4* factors = reinterpret_cast<float4*>(ws + 3 * x_bytes + 2 * a_bytes + sum_bytes + exp_bytes);
     double* part = reinterpret_cast<double*>(ws + 3 * x_bytes + 2 * a_bytes + sum_bytes + exp_bytes + factor_bytes);
+    float* S = reinterpret_cast<float*>(ws + 3 * x_bytes + 2 * a_bytes + sum_bytes + exp_bytes + factor_bytes + part_bytes);
     const T* G = static_cast<const T*>(p.G) + p.offG;
 
     const size_t tl = (p.len + 63) / 64, tiles = tl * ((p.lines + 63) / 64);
@@ -471,8 +530,15 @@ cudaError_t orthogonalize_typed(const OrthProblem& p, cudaStream_t s)
         __half* x = hi[k & 1];
         const Operand ox{x, m, n, ldx, xs}, oa{A, n, n, ldn, as}, op{P, n, n, ldn, as};
         Shape sq = {};
-        sq.U = sq.V = (unsigned)n; sq.K = (unsigned)m; sq.batch = (unsigned)batch; sq.tri = 1;
-        e = run_planned<KIND_F16, false>(ox, ox, sq, EpiGram{A, ldn, as, sizes}, s);
+        sq.U = sq.V = (unsigned)n; sq.batch = (unsigned)batch; sq.tri = 1;
+        for (size_t at = 0; at < m && e == cudaSuccess; at += SEGMENT) {
+            const size_t length = std::min(SEGMENT, m - at);
+            const Operand part{x + at, length, n, ldx, xs};
+            sq.K = (unsigned)length;
+            if (m <= SEGMENT) e = run_planned<KIND_F16, false>(part, part, sq, EpiGram<false>{A, ldn, as, sizes, nullptr}, s);
+            else if (at + length < m) e = run_planned<KIND_F16, false>(part, part, sq, EpiGramPart{S, ldn, as, at == 0}, s);
+            else e = run_planned<KIND_F16, false>(part, part, sq, EpiGram<true>{A, ldn, as, sizes, S}, s);
+        }
         plans[0] = last_plan();
         if (e == cudaSuccess && c != 0.f) {
             sq.K = (unsigned)n;

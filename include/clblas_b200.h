@@ -487,8 +487,9 @@ clblasStatus clblasB200I8gemm(
  *      power of two of its own, so a G whose norm is far below 1e-7 keeps the accuracy above.
  *      O may be G itself (BF16, same offset, pitch and stride); they may not overlap otherwise.  Matrices of G may overlap
  *      one another (strideG 0: one gradient), matrices of O may not.
- *      Workspace (from the library's pool): about 6 bytes per element of G and 4 per element of the smaller square; none where
- *      the smaller side is at most 128 and the larger at most 1024, or at most 2048 for at most 15 matrices.
+ *      Workspace (from the library's pool): about 6 bytes per element of G and 4 (8 where the larger side is above 131072)
+ *      per element of the smaller square; none where the smaller side is at most 128 and the larger at most 1024, or at
+ *      most 2048 for at most 15 matrices.
  *      Checks: G (A's status codes), O (C's; clblasInvalidLeadDimC also for a stride that makes its matrices overlap).
  *      A side of 2^31 and more is clblasNotImplemented; batchCount is as large as the buffers. */
 clblasStatus clblasB200Orthogonalize(
