@@ -1,7 +1,8 @@
 // Symmetric 8-bit quantisation with one scale per row or column (the operands of the 8-bit product):
 //   s = max|x| / 127,  q = rint(x * (127 / max|x|)),  x ~ s q.
 // Every operation is one IEEE FP32 operation, so the result does not depend on the launch.  Lines whose largest magnitude is below
-// 2^-100 (where 127 / max|x| would leave the range of FP32) count as zero: s = 0, q = 0.  A line that holds a NaN or an
+// 2^-100 count as zero: s = 0, q = 0.  (127 / max|x| stays finite down to 2^-121; the limit is part of the operator's definition,
+// chosen with room to that.)  A line that holds a NaN or an
 // infinity gets s = NaN, q = 0: the product with it is NaN, as the product with the line itself would be.
 //
 // Bound by memory: each element is read once and one byte written.
