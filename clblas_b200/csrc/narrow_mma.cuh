@@ -6,7 +6,7 @@
 // 0 loads slabs of 128 bytes along k with TMA into a ring, warp 1 owns tensor memory and issues the MMAs, warps 2-9 are the
 // epilogue.  Two accumulators in tensor memory, so the epilogue of a tile runs under the products of the next.  Bound by what L2
 // feeds the SMs (about 13 TB/s measured; a 256 x 256 tile moves 64 KB per slab) and, over seconds, by the power cap: 8-bit 8192^3
-// 318 to 350 us alone, 402 to 416 us back to back (cuBLAS on the same GPU 377 and 439); FP16 gram product 4096 x 16384 182 to 205 us.
+// 318 to 354 us alone, 397 to 412 us back to back (cuBLAS on the same GPU 377 and 439); FP16 gram product 4096 x 16384 182 to 205 us.
 //
 // narrow_split_kernel: for products with fewer tiles than SMs.  The k range of a tile is cut over the CTAs of a cluster; the
 // partial accumulators meet in distributed shared memory (each rank sums a slice of the columns, in rank order, so

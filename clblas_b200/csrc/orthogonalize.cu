@@ -8,9 +8,9 @@
 // the tiles of one triangle, each result stored at both places.  (Matrices up to 128 x 1024, and up to 128 x 2048 where
 // there are at most 15, take one kernel instead of the chain: orthogonalize_small.cu.)
 //
-// Measured, five steps: 4096 x 16384 BF16 3.65 ms alone, 4.2 ms back to back under the power cap (Gram 205 us, square 61, update 410: the
-// tiles without their epilogues 329, the rest is the 8 bytes an element that X costs to read and write); twelve 768 x 768 FP32 265 us
-// (15, 17, 29 us a step); two 2601 x 1003 257 us; 256 x 1024 98 us, of which launches and first loads are most.
+// Measured, five steps: 4096 x 16384 BF16 4.1 to 4.3 ms back to back under the power cap (Gram 205 us, square 61, update 410: the
+// tiles without their epilogues 329, the rest is the 8 bytes an element that X costs to read and write); twelve 768 x 768 FP32 264 us
+// (15, 17, 29 us a step); two 2601 x 1003 256 us; 256 x 1024 96 us, of which launches and first loads are most.
 //
 // What is kept in how many bits, and why:
 //   * X is a pair of FP16 numbers, hi + lo (22 bits); a X uses the pair, the products use hi.  Singular values far below the
@@ -27,7 +27,7 @@
 //     product is therefore taken in segments, which are added up in ordinary FP32 (8 x 2^24: 1.9e-4).  X is held times 2^12, A and P times 2^8, so that the
 //     entries of large matrices (about 1/sqrt(m)) stay far above FP16's smallest numbers, and times a power of two for each matrix where
 //     the whole matrix is small (orthogonalize.cuh).  768 x 768, |G|_F = 1e-15: 32 % off without that power, 3.4e-4 with it.
-// The result is good to about 1e-3 and is therefore given in BF16 only.
+// The result is good to 2e-4 to 1e-3 and is therefore given in BF16 only.
 #include "orthogonalize.cuh"
 
 #include <algorithm>

@@ -350,8 +350,8 @@ cudaError_t quantize_typed(bool per_line, const T* X, size_t ldx, signed char* Q
     if (lines >= (1u << 31)) return cudaErrorNotSupported;
     count_launch();
     const unsigned grid = (unsigned)lines;
-    // 64 elements a thread in registers.  8192 x 8192 BF16: 33 us with 128 threads a line (6.1 TB/s, 94 % of a copy's rate), 36 with 64 or
-    // 256 of 32 elements each, 42 with 512; so as few threads as hold the line.
+    // 64 elements a thread in registers.  8192 x 8192 BF16: 34 to 36 us in a row with 128 threads a line (5.6 to 5.9 TB/s, 87 to 91 % of a
+    // copy's rate), 3 more with 64 or 256 of 32 elements each, 9 more with 512; so as few threads as hold the line.
     if (aligned16(X) && (ldx * sizeof(T)) % 16 == 0 && (reinterpret_cast<uintptr_t>(Q) | ldq) % V == 0) {
         if (len <= 128 * 64) return launch_chained(quantize_lines_kernel<T, 128, V, 64 / V>, dim3(grid), 128, s, X, ldx, Q, ldq, scale, len);
         return launch_chained(quantize_lines_kernel<T, 256, V, 64 / V>, dim3(grid), 256, s, X, ldx, Q, ldq, scale, len);
