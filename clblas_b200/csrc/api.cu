@@ -37,6 +37,15 @@ MemGetAddressRangeFn address_range_fn()
     return fn;
 }
 
+// The driver answers questions about a pointer only in a thread that has a context, which a thread gets from its first runtime call
+// that works on a device.  For one whose first call is this library's: makes the context of its current device (0, where it has
+// set none) current.
+bool bind_context()
+{
+    int d = 0;
+    return cudaGetDevice(&d) == cudaSuccess && cudaSetDevice(d) == cudaSuccess;
+}
+
 // Bytes available from `ptr` to the end of its allocation; false when the pointer is not a
 // device allocation known to the driver.
 bool bytes_after(const void* ptr, size_t* avail)
@@ -45,7 +54,8 @@ bool bytes_after(const void* ptr, size_t* avail)
     if (!fn) return false;
     unsigned long long base = 0;
     size_t size = 0;
-    if (fn(&base, &size, (unsigned long long)(uintptr_t)ptr) != 0) {
+    if (fn(&base, &size, (unsigned long long)(uintptr_t)ptr) != 0 &&
+        (!bind_context() || fn(&base, &size, (unsigned long long)(uintptr_t)ptr) != 0)) {
         cudaGetLastError();
         return false;
     }
@@ -747,7 +757,12 @@ int device_of(const void* ptr)
     }();
     constexpr int kDeviceOrdinal = 9;                      // CU_POINTER_ATTRIBUTE_DEVICE_ORDINAL
     int d = -1;
-    if (!fn || fn(&d, kDeviceOrdinal, (unsigned long long)(uintptr_t)ptr) != 0) return -1;
+    if (!fn || ptr == nullptr) return -1;
+    if (fn(&d, kDeviceOrdinal, (unsigned long long)(uintptr_t)ptr) != 0 &&
+        (!bind_context() || fn(&d, kDeviceOrdinal, (unsigned long long)(uintptr_t)ptr) != 0)) {
+        cudaGetLastError();
+        return -1;
+    }
     return d;
 }
 
