@@ -64,8 +64,11 @@ class Chain:
         self.qy2, self.sy2 = [torch.zeros_like(q) for q in self.qy], [torch.zeros_like(s) for s in self.sy]
 
     def run(self, wait):
+        self.queue((lambda st: (cb.check(st), torch.cuda.synchronize())) if wait else cb.check)
+        torch.cuda.synchronize()
+
+    def queue(self, done=cb.check):
         T, O, K = self.T, self.O, self.K
-        done = (lambda st: (cb.check(st), torch.cuda.synchronize())) if wait else cb.check
         product = lambda: done(cb.clblasB200I8gemm(0, 0, 1, T, O, K, 1.0, self.qx, 0, K, self.sx, 0, self.qw, 0, K, self.sw, 0, 0.0, BF16, self.y, 0, O))  # noqa: E731
         left = cb.clblasLeft
         for i in range(self.steps):
@@ -78,7 +81,6 @@ class Chain:
             product()
             done(cb.clblasB200QuantizeI8(0, self.side, T, O, BF16, self.y, 0, O, self.qy2[i], 0, O, self.sy2[i], 0))
             done(cb.clblasB200Orthogonalize(0, O, K, 1, 5, None, -0.02, BF16, self.g[i], 0, K, 0, 0.99, self.w, 0, K, 0))
-        torch.cuda.synchronize()
 
 
 @pytest.mark.gpu
