@@ -20,14 +20,19 @@
 //   * The Gram matrix is stored as A = X X' - t I, t its mean diagonal, and P = (b + 2 c t) A + c A^2; X <- (a + b t + c t^2) X + P X is the
 //     same polynomial.  Near the end X X' is close to I and b, c nearly cancel: rounding the small difference instead
 //     halves the error of the result (normal 768 x 768: 1.5e-3 without, 7e-4 with t; the final rounding to BF16 is 1.7e-3).
+//   * Of the coefficient of X in that form, kappa = b t + c t^2 stands for what the shift took from P, which meets hi alone.  On lo it is right
+//     where the singular values are near one, and wrong by kappa lo where X has no component: the rounding of X would appear in empty
+//     directions and grow by a in every step (rank 50 of 100: 5e-3 of the result after five steps, 6 % after seven, 70 % after nine).  So kappa
+//     multiplies lo only in the steps after which |a| multiplies to 4 at most, the last two of the default ones: 1.8e-3, 3.2e-3, 2.4e-3
+//     (and with it nowhere 1.8e-3, 3.3e-3, 2.4e-3, but 1.2e-3 instead of 7e-4 for a normal 256 x 1024).
 //   * t comes from the sum of the squares of X, gathered in 64-bit integers (units of 2^-24), so the order of the atomic additions does
 //     not change it.  Any t gives the same polynomial; it only has to be near.
 //   * Accumulators and everything between accumulator and store are FP32.  The tensor core cuts its sums off instead of rounding them, so a
 //     long one falls behind, by about 2^-25 for every 16 terms (8 x 2^20: 1.5e-3 of the result, 8 x 2^24: 2.3 %).  Beyond SEGMENT elements the Gram
 //     product is therefore taken in segments, which are added up in ordinary FP32 (8 x 2^24: 1.9e-4).  X is held times 2^12, A and P times 2^8, so that the
 //     entries of large matrices (about 1/sqrt(m)) stay far above FP16's smallest numbers, and times a power of two for each matrix where
-//     the whole matrix is small (orthogonalize.cuh).  768 x 768, |G|_F = 1e-15: 32 % off without that power, 3.4e-4 with it.
-// The result is good to 2e-4 to 1e-3 and is therefore given in BF16 only.
+//     the whole matrix is small (orthogonalize.cuh).  768 x 768, |G|_F = 1e-15: 32 % off without that power, 1e-7 with it (before BF16).
+// The result is good to 3e-4 to 2e-3 after five steps and is therefore given in BF16 only.
 #include "orthogonalize.cuh"
 
 #include <algorithm>
@@ -194,10 +199,10 @@ __global__ void __launch_bounds__(256) split_kernel(const T* G, size_t lines, si
 // What the Gram product of a step finds and leaves for the others.
 struct Sizes {
     const u64* sums; int* exps;                            // sum of squares and exponent of every matrix before the step, `pitch` apart
-    float4* factors;                                       // of the step: b, f, w, g (StepFactors)
+    float4* factors;                                       // of the step, two each: (b, f) and (w, v, g) (StepFactors)
     int pitch;
     float n, a, b, c;
-    bool last;
+    bool last, kappa_lo;
     float scale;
 };
 
@@ -272,8 +277,9 @@ struct EpiGram {                                           // A <- X X' - t I
         st.t = SA * t;
         // Once for a matrix: evaluated by every tile of the products that need them they took 0.35 us a kernel.
         if (u0 == 0 && v0 == 0 && (threadIdx.x & 31) == 0) {
-            const StepFactors k = step_factors(mean * sizes.n, t, e, sizes.a, sizes.b, sizes.c, sizes.last, sizes.scale);
-            sizes.factors[at] = make_float4(k.b, k.f, k.w, k.g);
+            const StepFactors k = step_factors(mean * sizes.n, t, e, sizes.a, sizes.b, sizes.c, sizes.last, sizes.scale, sizes.kappa_lo);
+            sizes.factors[2 * at] = make_float4(k.b, k.f, 0.f, 0.f);
+            sizes.factors[2 * at + 1] = make_float4(k.w, k.v, k.g, 0.f);
             sizes.exps[at + 1] = k.next;
         }
     }
@@ -310,7 +316,7 @@ struct EpiSquare {                                         // P <- (b + 2 c t) A
     const float4* factors; int pitch;
     __device__ void begin(State& st, const Shape&, unsigned z, unsigned, unsigned) const
     {
-        const float4 k = __ldcg(factors + (size_t)z * pitch);
+        const float4 k = __ldcg(factors + 2 * (size_t)z * pitch);
         st.b = k.x;
         st.f = k.y;
     }
@@ -343,7 +349,7 @@ struct UpdateTerm {
     const __half* hi; const __half* lo; size_t ld, stride;
     const float4* factors; int pitch;
     template <int G> struct Pre { Bits16<G> h, l; };
-    struct Factors { float w, g; };                        // of X and of the product
+    struct Factors { float w, v, g; };                     // of hi, of lo and of the product
     template <int G>
     __device__ void fetch(Pre<G>& p, const Shape& s, unsigned z, unsigned u0, unsigned v0) const
     {
@@ -352,8 +358,8 @@ struct UpdateTerm {
     }
     __device__ Factors of(unsigned z) const
     {
-        const float4 k = __ldcg(factors + (size_t)z * pitch);
-        return {k.z, k.w};
+        const float4 k = __ldcg(factors + 2 * (size_t)z * pitch + 1);
+        return {k.x, k.y, k.z};
     }
     template <int G>
     __device__ void add(Pre<G>& p, const Shape& s, unsigned v0, const Factors& by, float (&x)[4][G][2]) const
@@ -365,8 +371,8 @@ struct UpdateTerm {
 #pragma unroll
             for (int k = 0; k < G; k++) {
                 const float2 h = unpack(p.h.h[g][k]), l = unpack(p.l.h[g][k]);
-                x[g][k][0] = fmaf(by.w, h.x + l.x, by.g * x[g][k][0]);
-                x[g][k][1] = fmaf(by.w, h.y + l.y, by.g * x[g][k][1]);
+                x[g][k][0] = fmaf(by.w, h.x, fmaf(by.v, l.x, by.g * x[g][k][0]));
+                x[g][k][1] = fmaf(by.w, h.y, fmaf(by.v, l.y, by.g * x[g][k][1]));
             }
     }
 };
@@ -493,7 +499,7 @@ cudaError_t orthogonalize_typed(const OrthProblem& p, cudaStream_t s)
     const size_t blocks = (p.lines * ((p.len + 7) / 8) + 2047) / 2048, most = std::max<size_t>(1, 2 * (size_t)sm_count() / batch);
     const size_t parts = std::min(blocks, most);
     // workspace: hi (two of them, read and written in turn), lo, A, P, sums of squares, exponents, factors, partial norms, sums of segments
-    const size_t x_bytes = up(batch * xs * 2, 256), a_bytes = up(batch * as * 2, 256), sum_bytes = up(batch * pitch * 8, 256), exp_bytes = up(batch * pitch * 4, 256), factor_bytes = up(batch * pitch * 16, 256),
+    const size_t x_bytes = up(batch * xs * 2, 256), a_bytes = up(batch * as * 2, 256), sum_bytes = up(batch * pitch * 8, 256), exp_bytes = up(batch * pitch * 4, 256), factor_bytes = up(batch * pitch * 32, 256),
                  part_bytes = up(batch * parts * 8, 256), join_bytes = m > SEGMENT ? batch * as * 4 : 0;
     unsigned char* ws = nullptr;
     cudaError_t e = ws_alloc(reinterpret_cast<void**>(&ws), 3 * x_bytes + 2 * a_bytes + sum_bytes + exp_bytes + factor_bytes + part_bytes + join_bytes, s);
@@ -526,7 +532,7 @@ cudaError_t orthogonalize_typed(const OrthProblem& p, cudaStream_t s)
     const char* plans[2] = {"", "none"};                   // of the last step's products
     for (int k = 0; k < p.steps && e == cudaSuccess; k++) {
         const float a = p.coeffs ? p.coeffs[3 * k] : 3.4445f, b = p.coeffs ? p.coeffs[3 * k + 1] : -4.7750f, c = p.coeffs ? p.coeffs[3 * k + 2] : 2.0315f;
-        const Sizes sizes{sums + k, exps + k, factors + k, pitch, (float)n, a, b, c, k + 1 == p.steps, p.alpha / SX};
+        const Sizes sizes{sums + k, exps + k, factors + 2 * k, pitch, (float)n, a, b, c, k + 1 == p.steps, kappa_on_lo(n, p.coeffs, k, p.steps), p.alpha / SX};
         __half* x = hi[k & 1];
         const Operand ox{x, m, n, ldx, xs}, oa{A, n, n, ldn, as}, op{P, n, n, ldn, as};
         Shape sq = {};
@@ -542,13 +548,13 @@ cudaError_t orthogonalize_typed(const OrthProblem& p, cudaStream_t s)
         plans[0] = last_plan();
         if (e == cudaSuccess && c != 0.f) {
             sq.K = (unsigned)n;
-            e = run_planned<KIND_F16, false>(oa, oa, sq, EpiSquare{A, P, ldn, as, factors + k, pitch}, s);
+            e = run_planned<KIND_F16, false>(oa, oa, sq, EpiSquare{A, P, ldn, as, factors + 2 * k, pitch}, s);
             plans[1] = last_plan();
         }
         if (e != cudaSuccess) break;
         Shape up_ = {};
         up_.U = (unsigned)n; up_.V = (unsigned)m; up_.K = (unsigned)n; up_.batch = (unsigned)batch;
-        const UpdateTerm t{x, lo, ldx, xs, factors + k, pitch};
+        const UpdateTerm t{x, lo, ldx, xs, factors + 2 * k, pitch};
         if (k + 1 < p.steps) {
             e = run_planned<KIND_F16, true>(c != 0.f ? op : oa, ox, up_, EpiUpdate{t, hi[(k + 1) & 1], lo, sums + k + 1}, s);
         } else {

@@ -4,6 +4,8 @@
 
 #include "narrow_mma.cuh"
 
+#include <cmath>
+
 namespace cb200 {
 
 // One cluster per matrix, everything on chip (orthogonalize_small.cu).
@@ -88,16 +90,16 @@ __device__ __forceinline__ void norm_factors(double norm, float& f0, float& f1, 
 }
 
 // The shift: the mean diagonal of Y Y' once most singular values of X have come near one; 0 before (and for a matrix of NaN, whose sum says
-// nothing).  While X is dominated by a few directions the shift would put roundings of t on all the others (rank 8 of 100: 3e-3
-// with t from the first step on, 7e-4 from t = 0.2 on).
+// nothing).
 __device__ __forceinline__ float shift(float mean, int e) { return (e == 0 ? mean : ldexpf(mean, -2 * e)) >= 0.2f ? mean : 0.f; }
 
-// A step in terms of what is stored: P <- b A + f A A, Y <- w Y + g P Y (A in place of P when c == 0); next: the exponent of X after it.
-struct StepFactors { float b, f, w, g; int next; };
+// A step in terms of what is stored: P <- b A + f A A, Y <- w hi + v lo + g P hi (A in place of P when c == 0); next: the exponent of X after
+// it.  Of w, kappa = b t + c t^2 is what the shift took from P.
+struct StepFactors { float b, f, w, v, g; int next; };
 
 // q2: |Y|^2, t: the shift.  The bounds, q = |X|_F: |X after the step|_F <= |a| q + |b| q^3 + |c| q^5, |P| <= 3 (|b| q^2 + |c| q^4) whatever t.
 // Not inlined: the kernel for small matrices has no registers to spare for it.
-__device__ __noinline__ StepFactors step_factors_scaled(float q2, float t, int e, float a, float b, float c, bool last, float scale)
+__device__ __noinline__ StepFactors step_factors_scaled(float q2, float t, int e, float a, float b, float c, bool last, float scale, bool kappa_lo)
 {
     const float grown = fabsf(b) * q2 + ldexpf(fabsf(c) * q2 * q2, -2 * e);                    // 4^e (|b| q^2 + |c| q^4)
     const float bound = sqrtf(q2) * (fabsf(a) + ldexpf(grown, -2 * e));                        // 2^e of the bound of X
@@ -109,19 +111,30 @@ __device__ __noinline__ StepFactors step_factors_scaled(float q2, float t, int e
     s.f = cp / SA;
     const int by = last ? -e : s.next - e;
     s.w = ldexpf(scale, by) * (a + t * (ldexpf(b, -2 * e) + ldexpf(c, -4 * e) * t));
+    s.v = kappa_lo ? s.w : ldexpf(scale, by) * a;
     s.g = ldexpf(scale * ((c == 0.f ? b : 1.f) / SA), by - (c == 0.f ? 2 * e : p));
     return s;
 }
 
-// In the last step Y is left times `scale` (alpha / SX) and without its power of two.
-__device__ __forceinline__ StepFactors step_factors(float q2, float t, int e, float a, float b, float c, bool last, float scale)
+// In the last step Y is left times `scale` (alpha / SX) and without its power of two.  kappa_lo: kappa multiplies lo too (orthogonalize.cu).
+__device__ __forceinline__ StepFactors step_factors(float q2, float t, int e, float a, float b, float c, bool last, float scale, bool kappa_lo)
 {
     if (!last) scale = 1.f;
     // The same without powers of two: the rule for gradients of ordinary size.
     const float grown = fabsf(b) * q2 + fabsf(c) * q2 * q2, sum = fabsf(a) + grown;
     if (e == 0 && grown >= 0.5f && q2 * sum * sum >= 0.25f)
-        return {b + 2.f * c * t, c / SA, scale * (a + t * (b + c * t)), scale * ((c == 0.f ? b : 1.f) / SA), 0};
-    return step_factors_scaled(q2, t, e, a, b, c, last, scale);
+        return {b + 2.f * c * t, c / SA, scale * (a + t * (b + c * t)), scale * (kappa_lo ? a + t * (b + c * t) : a), scale * ((c == 0.f ? b : 1.f) / SA), 0};
+    return step_factors_scaled(q2, t, e, a, b, c, last, scale, kappa_lo);
+}
+
+// Whether a step may put kappa on lo (orthogonalize.cu): what it leaves in empty directions grows by |a| in every step after it.  A matrix
+// of one row has none.
+inline bool kappa_on_lo(size_t n, const float* coeffs, int step, int steps)
+{
+    if (n == 1) return true;
+    float growth = 1.f;
+    for (int k = step + 1; k < steps; k++) growth *= fabsf(coeffs ? coeffs[3 * k] : 3.4445f);
+    return growth <= 4.f;
 }
 
 }  // namespace

@@ -33,6 +33,7 @@ struct SmallParams {
     uint16_t* O; size_t ldo, strideO;                          // BF16
     float alpha, beta;
     unsigned n, m, W;                                          // W: columns per CTA, a multiple of 64
+    u64 kappa_lo;                                              // bit k: step k puts kappa on lo
     int steps, align, align_g;                                 // align: of O's lines; align_g: of G's, 16, 4 or 2 bytes (16-bit types), 8 or 4 (FP32)
     bool flip;                                                 // X(u, v) at G[v * ldg + u] and O[v * ldo + u]
     float coeffs[3 * MAX_STEPS];
@@ -286,7 +287,7 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) orthogonalize_small_kernel(c
                 umma_commit<1>(bar);
             }
             __syncwarp();
-            by = step_factors(mean * (float)p.n, t, e, a, b, c, last, p.alpha / SX);       // under the products
+            by = step_factors(mean * (float)p.n, t, e, a, b, c, last, p.alpha / SX, (p.kappa_lo >> step) & 1);       // under the products
             wait_products();
 #pragma unroll
             for (int i = 0; i < 2; i++) {
@@ -321,7 +322,7 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) orthogonalize_small_kernel(c
             umma_commit<1>(bar);
         }
         __syncwarp();
-        if (c == 0.f) by = step_factors(mean * (float)p.n, t, e, a, b, c, last, p.alpha / SX);
+        if (c == 0.f) by = step_factors(mean * (float)p.n, t, e, a, b, c, last, p.alpha / SX, (p.kappa_lo >> step) & 1);
         wait_products();
         e = by.next;
         float total = 0;
@@ -338,7 +339,7 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) orthogonalize_small_kernel(c
                 for (int k = 0; k < 4; k++) {
                     uint32_t* xs = reinterpret_cast<uint32_t*>(X + slab_at(row0 + 8 * g, ch * 32 + 8 * k + 2 * q));
                     const float2 h = unpack(*xs), l = unpack(lo[i][g][k]);
-                    const float y0 = fmaf(by.w, h.x + l.x, by.g * x[g][k][0]), y1 = fmaf(by.w, h.y + l.y, by.g * x[g][k][1]);
+                    const float y0 = fmaf(by.w, h.x, fmaf(by.v, l.x, by.g * x[g][k][0])), y1 = fmaf(by.w, h.y, fmaf(by.v, l.y, by.g * x[g][k][1]));
                     x[g][k][0] = y0;
                     x[g][k][1] = y1;
                     if (!last) {
@@ -454,6 +455,7 @@ cudaError_t orthogonalize_small(const OrthProblem& p, cudaStream_t s)
     k.G = static_cast<const T*>(p.G) + p.offG; k.ldg = p.ldg; k.strideG = p.strideG;
     k.O = static_cast<uint16_t*>(p.O) + p.offO; k.ldo = p.ldo; k.strideO = p.strideO;
     k.alpha = p.alpha; k.beta = p.beta; k.steps = p.steps;
+    for (int i = 0; i < p.steps; i++) k.kappa_lo |= (u64)kappa_on_lo(k.n, p.coeffs, i, p.steps) << i;
     const size_t stride_g = p.batch > 1 ? p.strideG : 0;
     k.align_g = sizeof(T) == 2 ? line_alignment(k.G, p.ldg, stride_g)
                                : (reinterpret_cast<uintptr_t>(k.G) | p.ldg * 4 | stride_g * 4) % 8 == 0 ? 8 : 4;

@@ -30,10 +30,11 @@ def truncating_product(a, b):
     return acc
 
 
-def orth_emulated(g, coefficients, shift=True, low=True, gram=half, scaled=True, mul=product):
+def orth_emulated(g, coefficients, shift=True, low=True, gram=half, scaled=True, spread=False, mul=product):
     """NS(G), rows x cols, as the operator rounds it: X = hi + lo in two FP16 numbers times 2^e, the products take hi, the Gram matrix
-    minus its mean diagonal and the polynomial are FP16; sums are exact here.  The switches leave out what the design rests on
-    (the shift, the low half, FP16 for the Gram matrix, the power of two), for tests of the tests; mul: how products are summed."""
+    minus its mean diagonal and the polynomial are FP16; what the shift takes from the polynomial goes to hi, and to lo in the steps after which
+    |a| multiplies to 4 at most; sums are exact here.  The switches leave out what the design rests on (the shift, the low half, FP16
+    for the Gram matrix, the power of two, the last rule), for tests of the tests; mul: how products are summed."""
     g = g.double()
     flip = g.shape[0] > g.shape[1]
     if flip:
@@ -56,7 +57,9 @@ def orth_emulated(g, coefficients, shift=True, low=True, gram=half, scaled=True,
         P = half(2.0 ** p * ((bk + 2 * ck * t) * A + (ck / SA) * mul(A, A))) * 2.0 ** -p if c else bk * A
         bound = math.sqrt(q2) * (abs(a) + grown * 4.0 ** -e)
         after = max(0, e - exponent_of(bound)) if scaled and bound > 0 else e
-        y = ((a + t * (bk + ck * t)) * (hi + lo) + mul(P, hi) / SA) * 2.0 ** (after - e)
+        kappa = t * (bk + ck * t)
+        growth = math.prod(abs(x[0]) for x in coefficients[k + 1:])
+        y = ((a + kappa) * hi + (a + kappa if spread or growth <= 4 or n == 1 else a) * lo + mul(P, hi) / SA) * 2.0 ** (after - e)
         e = after
     x = y / SX * 2.0 ** -e
     return x.t() if flip else x
