@@ -251,8 +251,8 @@ void ws_release_all();
 // through ws_alloc, so a call during which this does not move allocated nothing).
 unsigned long long ws_alloc_count();
 
-// Set-up steps that are no stream work (creating a pool, a kernel's attributes) may fall into a call that is being captured; in
-// the relaxed mode they neither fail nor spoil the capture.  Holds for the calling thread while it lives.
+// Set-up steps that are no stream work (creating a pool, a kernel's attributes) may fall into a call that is being captured, or into one
+// beside another thread's capture, and so may workspaces; in the relaxed mode they neither fail nor spoil the capture.  Holds for the calling thread while it lives.
 struct RelaxedCapture {
     cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
     RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }

@@ -48,12 +48,19 @@ cudaError_t ws_alloc(void** ptr, size_t bytes, cudaStream_t s)
     cudaMemPool_t pool;
     cudaError_t e = pool_for_current_device(&pool);
     if (e != cudaSuccess) return e;
+    // While any thread captures in the global mode (the usual one) this call counts as unsafe in all others, and would end that capture
+    // as well as fail.  It is ordered on its own stream and touches no other.
+    RelaxedCapture relaxed;
     return cudaMallocFromPoolAsync(ptr, bytes, pool, s);
 }
 
 unsigned long long ws_alloc_count() { return g_allocs.load(std::memory_order_relaxed); }
 
-cudaError_t ws_free(void* ptr, cudaStream_t s) { return cudaFreeAsync(ptr, s); }
+cudaError_t ws_free(void* ptr, cudaStream_t s)
+{
+    RelaxedCapture relaxed;
+    return cudaFreeAsync(ptr, s);
+}
 
 void ws_release_all()
 {

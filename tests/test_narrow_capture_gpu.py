@@ -1,4 +1,8 @@
-"""Narrow-type calls in CUDA graphs, without other kernels between them."""
+"""Narrow-type calls in CUDA graphs, without other kernels between them, and beside a capture of another thread."""
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -8,6 +12,7 @@ from tests.test_narrow_handover import Chain
 
 pytestmark = pytest.mark.gpu
 
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 BF16 = cb.clblasB200Bfloat16
 
 
@@ -75,3 +80,49 @@ def test_two_graphs_with_workspaces_at_once():
     torch.cuda.synchronize()
     for z, w in zip(sets, want):
         assert all(torch.equal(t, v) for t, v in zip((z[2], z[3], z[5], z[6]), w))
+
+
+OTHER_THREAD = """
+import sys, threading, torch, clblas_b200 as cb
+def make(seed):
+    gen = torch.Generator(device='cuda').manual_seed(seed)
+    x = torch.randn(4608, 4096, generator=gen, device='cuda').bfloat16()
+    a = torch.randint(-127, 128, (40, 4608), generator=gen, device='cuda', dtype=torch.int32).to(torch.int8)
+    g, m = torch.randn(300, 420, generator=gen, device='cuda'), torch.randn(200, 300, generator=gen, device='cuda')
+    t = torch.eye(200, device='cuda') * 16 + torch.randn(200, 200, generator=gen, device='cuda').tril()
+    return (x, a, g, t, m), (torch.zeros_like(x, dtype=torch.int8), torch.zeros(4096, device='cuda'), torch.zeros(40, 4096, device='cuda'),
+                          torch.zeros(300, 420, dtype=torch.bfloat16, device='cuda'))
+def calls(z, stream):
+    (x, a, g, t, m), (q, s, c, o) = z
+    k = dict(queues=[stream])
+    return [cb.clblasB200QuantizeI8(0, 1, 4608, 4096, 2, x, 0, 4096, q, 0, 4096, s, 0, **k),
+            cb.clblasB200I8gemm(0, 0, 0, 40, 4096, 4608, 1.0, a, 0, 4608, None, 0, q, 0, 4096, s, 0, 0.0, 0, c, 0, 4096, **k),
+            cb.clblasB200Orthogonalize(0, 300, 420, 1, 5, None, 1.0, 0, g, 0, 420, 0, 0.0, o, 0, 420, 0, **k),
+            cb.clblasStrsm(0, 0, 1, 0, 1, 200, 300, 1.0, t, 0, 200, m, 0, 300, **k)]
+assert cb.clblasSetup() == 0
+a, b, want = make(1), make(2), make(2)
+streams = [torch.cuda.Stream() for _ in range(2)]
+torch.cuda.synchronize()
+if sys.argv[1] == 'warm':
+    assert calls(make(3), streams[0]) == [0] * 4
+    torch.cuda.synchronize()
+got, graph = [], torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph, stream=streams[0]):               # the global mode: nothing unsafe in any thread
+    t = threading.Thread(target=lambda: got.append(calls(b, streams[1])))
+    t.start(); t.join()
+    got.append(calls(a, streams[0]))
+graph.replay()
+assert calls(want, streams[1]) == [0] * 4
+torch.cuda.synchronize()
+assert got == [[0] * 4] * 2, got
+assert all(torch.equal(u, v) for u, v in zip(b[1], want[1])) and torch.equal(b[0][4], want[0][4])
+assert int(a[1][0].abs().max()) == 127 and 15 < float(a[1][3].float().norm()) < 21
+print('captured beside another thread')
+"""
+
+
+@pytest.mark.parametrize("state", ["cold", "warm"])
+def test_calls_beside_another_threads_capture(state):
+    """One thread captures while another makes calls with workspaces on a stream of its own: neither disturbs the other."""
+    r = subprocess.run([sys.executable, "-c", OTHER_THREAD, state], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured beside another thread" in r.stdout, r.stderr[-2000:]
