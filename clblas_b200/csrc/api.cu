@@ -46,20 +46,49 @@ bool bind_context()
     return cudaGetDevice(&d) == cudaSuccess && cudaSetDevice(d) == cudaSuccess;
 }
 
-// Bytes available from `ptr` to the end of its allocation; false when the pointer is not a
-// device allocation known to the driver.
-bool bytes_after(const void* ptr, size_t* avail)
+// Whether an address lies in memory mapped by cuMemMap (an allocator with growing segments).
+bool mapped_memory(unsigned long long address)
+{
+    typedef int (*RetainFn)(unsigned long long*, void*);
+    typedef int (*ReleaseFn)(unsigned long long);
+    struct Functions {
+        RetainFn retain = nullptr;
+        ReleaseFn release = nullptr;
+        Functions()
+        {
+            void *f = nullptr, *g = nullptr;
+            cudaDriverEntryPointQueryResult q;
+            if (cudaGetDriverEntryPoint("cuMemRetainAllocationHandle", &f, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) return;
+            if (cudaGetDriverEntryPoint("cuMemRelease", &g, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) return;
+            retain = reinterpret_cast<RetainFn>(f);
+            release = reinterpret_cast<ReleaseFn>(g);
+        }
+    };
+    static const Functions fn;
+    unsigned long long handle = 0;
+    if (!fn.retain || fn.retain(&handle, reinterpret_cast<void*>(address)) != 0) return false;
+    fn.release(handle);
+    return true;
+}
+
+// Bytes available from `ptr` to the end of its allocation; false when the pointer is not a device allocation known to the driver.
+// Memory mapped by cuMemMap is known to the driver in pieces, as it was mapped; where `need` bytes are more than the first has, the
+// pieces that follow without a gap count too.
+bool bytes_after(const void* ptr, size_t need, size_t* avail)
 {
     MemGetAddressRangeFn fn = address_range_fn();
     if (!fn) return false;
     unsigned long long base = 0;
     size_t size = 0;
-    if (fn(&base, &size, (unsigned long long)(uintptr_t)ptr) != 0 &&
-        (!bind_context() || fn(&base, &size, (unsigned long long)(uintptr_t)ptr) != 0)) {
+    const unsigned long long address = (unsigned long long)(uintptr_t)ptr;
+    if (fn(&base, &size, address) != 0 && (!bind_context() || fn(&base, &size, address) != 0)) {
         cudaGetLastError();
         return false;
     }
-    *avail = size - (size_t)((unsigned long long)(uintptr_t)ptr - base);
+    unsigned long long end = base + size;
+    if (end - address < need && mapped_memory(address))
+        while (end - address < need && mapped_memory(end) && fn(&base, &size, end) == 0 && base == end) end += size;
+    *avail = (size_t)(end - address);
     return true;
 }
 
@@ -76,6 +105,12 @@ bool extent_fits(size_t off, size_t lines, size_t len, size_t ld, size_t have)
 {
     return off <= have && len <= have - off && (lines - 1) <= (have - off - len) / ld;
 }
+// The bytes of such an extent; all of the address space where that is less.
+size_t extent_bytes(size_t off, size_t lines, size_t len, size_t ld, size_t tsize)
+{
+    const unsigned __int128 elements = (unsigned __int128)(lines - 1) * ld + len + off, most = SIZE_MAX / tsize;
+    return (size_t)(elements < most ? elements : most) * tsize;
+}
 
 // checkMatrixSizes of the reference (src/library/blas/generic/common.c:585-686) for a non-packed
 // rows x cols matrix op(X).
@@ -88,7 +123,7 @@ clblasStatus check_matrix_sizes(size_t tsize, clblasOrder order, clblasTranspose
     const size_t lines = tra ? cols : rows, len = tra ? rows : cols;
     if (ld < len) return pick(e, clblasInvalidLeadDimA, clblasInvalidLeadDimB, clblasInvalidLeadDimC);
     size_t avail = 0;
-    if (!bytes_after(buf, &avail)) return pick(e, clblasInvalidMatA, clblasInvalidMatB, clblasInvalidMatC);
+    if (!bytes_after(buf, extent_bytes(off, lines, len, ld, tsize), &avail)) return pick(e, clblasInvalidMatA, clblasInvalidMatB, clblasInvalidMatC);
     if (!extent_fits(off, lines, len, ld, avail / tsize))
         return pick(e, clblasInsufficientMemMatA, clblasInsufficientMemMatB, clblasInsufficientMemMatC);
     return clblasSuccess;
@@ -789,7 +824,7 @@ bool on_other_device(const void* ptr, int device)
 clblasStatus check_f32_vector(const void* buf, size_t off, size_t n, int device, clblasStatus invalid, clblasStatus insufficient)
 {
     size_t avail = 0;
-    if (buf == nullptr || !bytes_after(buf, &avail) || on_other_device(buf, device)) return invalid;
+    if (buf == nullptr || !bytes_after(buf, extent_bytes(off, 1, n, n, 4), &avail) || on_other_device(buf, device)) return invalid;
     return off > avail / 4 || n > avail / 4 - off ? insufficient : clblasSuccess;
 }
 
@@ -874,8 +909,10 @@ clblasStatus check_batch_extent(size_t tsize, size_t lines, size_t len, const vo
                                 clblasStatus insufficient)
 {
     size_t avail = 0;
-    if (batch > 1 && (!bytes_after(buf, &avail) || stride > avail / tsize / (batch - 1) ||
-                      off + (batch - 1) * stride + (lines - 1) * ld + len > avail / tsize))
+    if (batch <= 1) return clblasSuccess;
+    const unsigned __int128 first = extent_bytes(off, lines, len, ld, tsize), whole = first + (unsigned __int128)(batch - 1) * stride * tsize;
+    if (!bytes_after(buf, whole < SIZE_MAX ? (size_t)whole : SIZE_MAX, &avail) || stride > avail / tsize / (batch - 1) ||
+        off + (batch - 1) * stride + (lines - 1) * ld + len > avail / tsize)
         return insufficient;
     return clblasSuccess;
 }
