@@ -24,7 +24,9 @@
 //     where the singular values are near one, and wrong by kappa lo where X has no component: the rounding of X would appear in empty
 //     directions and grow by a in every step (rank 50 of 100: 5e-3 of the result after five steps, 6 % after seven, 70 % after nine).  So kappa
 //     multiplies lo only in the steps after which |a| multiplies to 4 at most, the last two of the default ones: 1.8e-3, 3.2e-3, 2.4e-3
-//     (and with it nowhere 1.8e-3, 3.3e-3, 2.4e-3, but 1.2e-3 instead of 7e-4 for a normal 256 x 1024).
+//     (and with it nowhere 1.8e-3, 3.3e-3, 2.4e-3, but 1.2e-3 instead of 7e-4 for a normal 256 x 1024).  Where all singular values lie close
+//     together kappa on lo would be right throughout (a normal 64 x 8192: 2e-4 instead of 9e-4); asking |X X' - t I|_F^2 < t^2, which
+//     tells those apart, cost 2 to 6 % of the kernel for small matrices and is hidden by the rounding to BF16, 1.7e-3.
 //   * t comes from the sum of the squares of X, gathered in 64-bit integers (units of 2^-24), so the order of the atomic additions does
 //     not change it.  Any t gives the same polynomial; it only has to be near.
 //   * Accumulators and everything between accumulator and store are FP32.  The tensor core cuts its sums off instead of rounding them, so a

@@ -53,7 +53,7 @@ __device__ __forceinline__ double sum_of_squares(const float (&x)[8])
 // coefficients a, 4^-e b, 16^-e c.  P, which is far smaller than X there, is held times 2^p in the same way.
 constexpr int MAX_EXPONENT = 300;
 
-// v = m 2^x with m in [0.5, 1): -x, within [0, MAX_EXPONENT]; 0 for 0 and for what is not finite.
+// v = m 2^x with m in [0.5, 1): plus - x, within [0, MAX_EXPONENT]; 0 for 0 and for what is not finite.
 __device__ __forceinline__ int raising(float v, int plus)
 {
     int x = 0;

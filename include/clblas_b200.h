@@ -481,8 +481,8 @@ clblasStatus clblasB200I8gemm(
  *      with (a, b, c) = coefficients[3k .. 3k+2] (host memory) in step k, or (3.4445, -4.7750, 2.0315) in every step when
  *      coefficients is NULL.  1 <= steps <= 64.
  *      G: FP32 / FP16 / BF16.  O: BF16 (the products take 11-bit operands: after five steps the result is good to about 1e-3
- *      relative to its own norm, 2e-3 where the rank is partial, 3e-3 for a few rows; the default coefficients do not
- *      converge but go on moving the singular values, so every two steps more may double that).  beta == 0 never reads O.  A G that holds a NaN or an infinity gives NaN everywhere.  The iteration
+ *      relative to its own norm, 2e-3 where the rank is partial, 5e-3 at worst below 16 rows; the default coefficients do
+ *      not converge but go on moving the singular values, so every two steps more may double that).  beta == 0 never reads O.  A G that holds a NaN or an infinity gives NaN everywhere.  The iteration
  *      runs in FP16 with scale factors that leave room for singular values of X up to 16 and for |b| s^2 + |c| s^4 up to 255
  *      at singular values s; coefficients that drive X further overflow.  There is no lower end: a small X is held times a
  *      power of two of its own, so a G whose norm is far below 1e-7 keeps the accuracy above.
